@@ -344,6 +344,37 @@ int asap_ffn_job_info(uint64_t ws_handle, int32_t* n, int32_t* layer_id, uint32_
 int asap_ffn_debug_ptrs(uint64_t ws_handle, uint64_t* expert_counts, uint64_t* pair_pos, uint64_t* xq,
                         uint64_t* xq_sf, uint64_t* hq, uint64_t* hq_sf, uint64_t* y2);
 
+/* ------------------------------------------------------------------ the attention rank's half of the layer
+ * FP8 block-scaled linear: W [n, k] E4M3 bytes (checkpoint order) with one fp32 scale per 128 x 128 block, [ceil(n /
+ * 128), ceil(k / 128)]; n and k multiples of 16 (the last blocks may be partial).  Activations are quantised per row
+ * and 128 values of K: scale = amax / 448, codes = e4m3(x * (448 / amax)); with pow2 the scale is rounded up to a power
+ * of two and codes = e4m3(x / scale) (for weights whose scales are E8M0, given here as the fp32 values they stand
+ * for). */
+#define ASAP_LINEAR_MAX_ROWS (1 << 20)
+#define ASAP_LINEAR_MAX_DIM (1 << 17)
+typedef struct {
+  int32_t n, k;
+  uint64_t w, scale;
+  int32_t pow2, pad;
+} asap_fp8_linear_t;
+int asap_fp8_linear_register(const asap_fp8_linear_t* d, uint64_t* handle);
+int asap_fp8_linear_release(uint64_t handle);
+
+/* out [m, n] = x W^T.  x [m, k] bf16 (fp16 != 0: half), rows ldx elements apart (a multiple of 8), 16-byte aligned;
+ * out of x's type, rows n apart.  ws: 256-byte aligned scratch of asap_fp8_linear_ws_bytes(m, k), free again when the
+ * call's work is done.  A pipeline wait that runs out reports to `status` (0: nowhere). */
+uint64_t asap_fp8_linear_ws_bytes(int32_t m, int32_t k);
+int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t fp16, uint64_t out, uint64_t ws,
+                    uint64_t ws_bytes, uint64_t status, uint64_t timeout_ns, void* stream);
+
+/* The shared expert: out [m, H] = (silu(g) * u) W2^T with [g, u] = x W13^T (w13 [2I, H]: gate rows, then up rows; w2
+ * [H, I]; I % 128 == 0; g clamped to at most and u to +-swiglu_limit when that is > 0).  h = silu(g) * u is
+ * requantised per row and 128 values in the first product's epilogue. */
+uint64_t asap_fp8_shared_ws_bytes(int32_t m, int32_t hidden, int32_t inter);
+int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t ldx, int32_t m, int32_t fp16,
+                    float swiglu_limit, uint64_t out, uint64_t ws, uint64_t ws_bytes, uint64_t status,
+                    uint64_t timeout_ns, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_uint8, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_uint8, c_uint32, c_uint64, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libasap.so")
 
@@ -51,6 +51,11 @@ class FfnRow_t(ctypes.Structure):
 class Fp8Experts_t(ctypes.Structure):
     _fields_ = [("num_local", c_int32), ("expert_base", c_int32), ("hidden", c_int32), ("inter", c_int32),
                 ("w13", c_uint64), ("w13_scale", c_uint64), ("w2", c_uint64), ("w2_scale", c_uint64)]
+
+
+class Fp8Linear_t(ctypes.Structure):
+    _fields_ = [("n", c_int32), ("k", c_int32), ("w", c_uint64), ("scale", c_uint64), ("pow2", c_int32),
+                ("pad", c_int32)]
 
 
 # name -> (restype, argtypes); every int-returning call is checked
@@ -122,6 +127,14 @@ _SIGS = {
     "asap_dispatch_info": (c_int32, [c_uint64, c_int32, POINTER(c_int32), POINTER(c_uint64), POINTER(c_uint64),
                                      c_void_p]),
     "asap_ffn_debug_ptrs": (c_int32, [c_uint64] + [POINTER(c_uint64)] * 7),
+    "asap_fp8_linear_register": (c_int32, [POINTER(Fp8Linear_t), POINTER(c_uint64)]),
+    "asap_fp8_linear_release": (c_int32, [c_uint64]),
+    "asap_fp8_linear_ws_bytes": (c_uint64, [c_int32, c_int32]),
+    "asap_fp8_linear": (c_int32, [c_uint64, c_uint64, c_int64, c_int32, c_int32, c_uint64, c_uint64, c_uint64, c_uint64,
+                                  c_uint64, c_void_p]),
+    "asap_fp8_shared_ws_bytes": (c_uint64, [c_int32, c_int32, c_int32]),
+    "asap_fp8_shared": (c_int32, [c_uint64, c_uint64, c_uint64, c_int64, c_int32, c_int32, c_float, c_uint64, c_uint64,
+                                  c_uint64, c_uint64, c_uint64, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,213 @@
+"""The dense FP8 products of an attention rank: a linear layer over block-scaled weights, and the shared expert.
+
+The checkpoints whose routed experts ``experts.Fp8Experts`` serves hold their dense weights in the same format: E4M3
+values with one scale per 128 x 128 block.  ``Fp8Linear`` multiplies by such a weight without widening it;
+``Fp8SharedExpert`` is the SwiGLU expert every token passes through, whose output the combine adds
+(``AsapDispatcher.combine(out, shared=...)``, ``AsapMoE.shared_expert``; the reference adds the shared output in
+python/sgl_asap_plugin/srt/batch_overlap/operations_strategy.py:106-111).
+
+    y[r, n] = sum_b sa[r, b] * sb[n // 128, b] * sum_{k in block b} xq[r, k] * w[n, k]
+
+Activations are quantised inside the call, per row and block b of 128 values along K:
+
+* fp32 weight scales: sa = amax / 448, xq = e4m3(x * (448 / amax)), the quotients and the product each rounded to fp32
+  (the rule of the routed experts' activations);
+* E8M0 weight scales (``torch.float8_e8m0fnu``): sa = amax / 448 rounded up to a power of two, xq = e4m3(x / sa).
+
+amax counts as at least 1e-10.  A NaN or infinity in a row makes that row of the result NaN and no other.  Sums are
+held in fp32 and rounded once to x's type.  Both are for serving: they have no gradient.  A call allocates its scratch
+from torch's caching allocator on the current stream, so calls on different streams and captured graphs share nothing.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _native as N
+
+TIMEOUT_NS = 5_000_000_000  # bound of every wait inside the kernels
+_status: dict = {}          # device index -> int64 status word
+
+
+def _status_word(device: torch.device) -> torch.Tensor:
+    word = _status.get(device.index)
+    if word is None:
+        word = _status[device.index] = torch.zeros(1, dtype=torch.int64, device=device)
+    return word
+
+
+def check(device: int = 0) -> None:
+    """Raise if a kernel of this module gave up a wait on ``device`` (synchronises it)."""
+    word = _status.get(device)
+    if word is not None:
+        torch.cuda.synchronize(device)
+        value = int(word.item())
+        if value:
+            word.zero_()
+            raise N.AsapError("asap_fp8_linear", N.ASAP_ETIMEOUT, f"device status {N.decode_status(value)}")
+
+
+class _Weight:
+    """A registered [n, k] weight (keeps its tensors alive)."""
+
+    def __init__(self, name: str, w: torch.Tensor, scale: torch.Tensor):
+        if w.dtype == torch.float8_e4m3fn:
+            w = w.view(torch.uint8)
+        if w.dtype != torch.uint8 or w.dim() != 2 or not w.is_contiguous():
+            raise ValueError(f"{name}: need contiguous E4M3 values [n, k] (float8_e4m3fn or their bytes), got "
+                             f"{w.dtype} {tuple(w.shape)}")
+        self.n, self.k = w.shape
+        if self.n < 16 or self.k < 16 or self.n % 16 or self.k % 16:
+            raise ValueError(f"{name}: n and k must be multiples of 16, got {self.n} x {self.k}")
+        blocks = (-(-self.n // 128), -(-self.k // 128))
+        if scale.dtype not in (torch.float32, torch.float8_e8m0fnu) or tuple(scale.shape) != blocks:
+            raise ValueError(f"{name}: need float32 or float8_e8m0fnu scales of shape {blocks}, got {scale.dtype} "
+                             f"{tuple(scale.shape)}")
+        if not w.is_cuda or scale.device != w.device:
+            raise ValueError(f"{name}: the weight and its scales must be on one CUDA device")
+        if w.data_ptr() % 16:
+            raise ValueError(f"{name}: the weight must be 16-byte aligned")
+        self.pow2 = scale.dtype == torch.float8_e8m0fnu
+        self.w, self.scale = w, scale.float().contiguous()
+        self.device = w.device
+        self.handle = 0
+        desc = N.Fp8Linear_t(self.n, self.k, self.w.data_ptr(), self.scale.data_ptr(), int(self.pow2), 0)
+        h = ctypes.c_uint64()
+        with torch.cuda.device(self.device):
+            N.call("asap_fp8_linear_register", ctypes.byref(desc), ctypes.byref(h))
+        self.handle = h.value
+        self.status = _status_word(self.device).data_ptr()
+
+    def release(self) -> None:
+        if self.handle:
+            handle, self.handle = self.handle, 0
+            N.call("asap_fp8_linear_release", handle)
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:  # noqa: BLE001  (interpreter shutdown)
+            pass
+
+
+def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int):
+    """-> (x as rows the kernels can read, their stride, out of x's leading shape)."""
+    if not weight.handle:
+        raise RuntimeError("the layer was released")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != weight.k or x.device != weight.device:
+        raise ValueError(f"x must be [..., {weight.k}] on {weight.device}, got {tuple(x.shape)} on {x.device}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("the FP8 products have no gradient: call them under torch.no_grad() or detach x")
+    shape = (*x.shape[:-1], n)
+    rows = x if x.dim() == 2 else x.reshape(-1, weight.k)
+    if rows.shape[0] > 1 << 20:
+        raise ValueError(f"at most {1 << 20} rows per call, got {rows.shape[0]}")
+    ld = rows.stride(0) if rows.shape[0] > 1 else weight.k
+    if (weight.k > 1 and rows.stride(1) != 1) or ld % 8 or ld < weight.k or rows.data_ptr() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        ld = weight.k
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif (out.dtype != x.dtype or tuple(out.shape) != shape or out.device != x.device or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {x.dtype} tensor of shape {shape} on {x.device}")
+    return rows, ld, out
+
+
+class _OnDevice:
+    """torch.cuda.device(index) that costs nothing when the device is the current one already."""
+
+    def __init__(self, device: torch.device):
+        self.index, self.prev = device.index, -1
+
+    def __enter__(self):
+        current = torch.cuda.current_device()
+        if current != self.index:
+            self.prev = current
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+class Fp8Linear:
+    """y = x W^T over an E4M3 weight [n, k] with one scale per 128 x 128 block, [ceil(n/128), ceil(k/128)], fp32 or
+    E8M0.  n and k are multiples of 16.  x: bf16 or fp16 [..., k] of any strides -> [..., n] of its type; ``out`` takes
+    the result in place of a new tensor."""
+
+    def __init__(self, weight: torch.Tensor, scale: torch.Tensor):
+        self._w = _Weight("weight", weight, scale)
+
+    @property
+    def shape(self) -> tuple:
+        return self._w.n, self._w.k
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor) -> "Fp8Linear":
+        """A dense CUDA weight [n, k] (multiples of 128) -> block-quantised (``quant.fp8_block_quantize``)."""
+        from .quant import fp8_block_quantize
+
+        return cls(*fp8_block_quantize(w))
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        w = self._w
+        rows, ld, out = _rows(x, w, out, w.n)
+        m = rows.shape[0]
+        if m:
+            nbytes = N.lib().asap_fp8_linear_ws_bytes(m, w.k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+            with _OnDevice(w.device):
+                N.call("asap_fp8_linear", w.handle, rows.data_ptr(), ld, m, int(x.dtype == torch.float16),
+                       out.data_ptr(), ws.data_ptr(), nbytes, w.status, TIMEOUT_NS,
+                       torch.cuda.current_stream(w.device).cuda_stream)
+        return out
+
+    def release(self) -> None:
+        self._w.release()
+
+
+class Fp8SharedExpert:
+    """out = (silu(g) * u) W2^T with [g, u] = x W13^T: w13 [2I, H] (gate rows, then up rows), w2 [H, I], both with
+    block scales as ``Fp8Linear`` takes them, of one kind; I a multiple of 128, H of 16.  ``swiglu_limit`` > 0 clamps g
+    to at most and u to +-that value.  h = silu(g) * u goes to the second product requantised per row and 128 values,
+    never through 16 bits."""
+
+    def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor, *,
+                 swiglu_limit: float = 0.0):
+        self._w13, self._w2 = _Weight("w13", w13, w13_scale), _Weight("w2", w2, w2_scale)
+        self.hidden, self.inter, self.swiglu_limit = self._w13.k, self._w2.k, float(swiglu_limit)
+        if (self._w13.n != 2 * self.inter or self._w2.n != self.hidden or self.inter % 128
+                or self._w13.device != self._w2.device or self._w13.pow2 != self._w2.pow2):
+            raise ValueError(f"need w13 [2I, H] and w2 [H, I] with I % 128 == 0, one device and one kind of scales, got "
+                             f"{self._w13.n} x {self._w13.k} and {self._w2.n} x {self._w2.k}")
+
+    @classmethod
+    def from_float(cls, w13: torch.Tensor, w2: torch.Tensor, *, swiglu_limit: float = 0.0) -> "Fp8SharedExpert":
+        """Dense CUDA weights w13 [2I, H] and w2 [H, I] (multiples of 128) -> block-quantised."""
+        from .quant import fp8_block_quantize
+
+        return cls(*fp8_block_quantize(w13), *fp8_block_quantize(w2), swiglu_limit=swiglu_limit)
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        a, b = self._w13, self._w2
+        rows, ld, out = _rows(x, a, out, b.n)
+        m = rows.shape[0]
+        if m:
+            nbytes = N.lib().asap_fp8_shared_ws_bytes(m, self.hidden, self.inter)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+            with _OnDevice(a.device):
+                N.call("asap_fp8_shared", a.handle, b.handle, rows.data_ptr(), ld, m, int(x.dtype == torch.float16),
+                       self.swiglu_limit, out.data_ptr(), ws.data_ptr(), nbytes, a.status, TIMEOUT_NS,
+                       torch.cuda.current_stream(a.device).cuda_stream)
+        return out
+
+    def release(self) -> None:
+        self._w13.release()
+        self._w2.release()
