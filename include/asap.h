@@ -375,6 +375,53 @@ int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t
                     float swiglu_limit, uint64_t out, uint64_t ws, uint64_t ws_bytes, uint64_t status,
                     uint64_t timeout_ns, void* stream);
 
+/* Router: the top-k experts of each token and their weights, as asap_dispatch takes them.  logits [t, e], rows ld
+ * elements apart, dtype 0 fp32, 1 bf16, 2 fp16.  Scores: softmax of the row, or sigmoids.  Selection by score + bias
+ * (fp32 [e]; 0: by score), exactly as unrounded arithmetic ranks them, ties to the lowest expert; with groups > 1 only
+ * among the top_groups best of `groups` equal runs of experts (a group's score: its best expert's, or with a bias the
+ * sum of its two best).  weight = scale * score [/ (sum of the selected scores + 1e-20)].  An expert whose logit (or
+ * bias) is -inf is never chosen; places left over get id -1, weight 0, and so do the rows from *num_tokens (int32 on the
+ * device; 0: t) on.  A NaN logit counts as -inf and makes the row's weights NaN. */
+#define ASAP_ROUTE_MAX_EXPERTS 1024
+#define ASAP_ROUTE_MAX_TOPK 32
+typedef struct {
+  uint64_t logits;
+  int64_t ld;
+  int32_t dtype, t, e, k;
+  int32_t sigmoid, groups, top_groups, renormalize;
+  float scale;
+  int32_t pad;
+  uint64_t bias, num_tokens;
+} asap_route_t;
+int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stream);
+
+/* d loss / d logits [t, e] of the logits' type, rows e apart, from grad_weights fp32 [t, k] and the ids asap_route
+ * chose (the selection itself has no gradient; the bias gets none). */
+int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weights, uint64_t grad_logits,
+                        void* stream);
+
+/* Balance loss of a choice of experts, per sequence: loss = coef * mean over the sequences with a live token of sum_e
+ * f_e P_e, f_e = e / (k n) * count_e, P_e = mean of p_te over the sequence's n live tokens (those with an id), p the
+ * row's softmax or its sigmoids normalised to sum 1.  ids int32 [t, k], -1: none.  cu_seqlens int32 [seqs + 1] on the
+ * device, from 0, not decreasing (0: one sequence); tokens behind the last sequence do not take part.  The workspace
+ * starts with the counts, int32 [seqs, e]; the gradient reads it again.  The loss is the same bits every time. */
+typedef struct {
+  uint64_t logits;
+  int64_t ld;
+  int32_t dtype, t, e, k;
+  int32_t sigmoid, seqs;
+  float coef;
+  int32_t pad;
+  uint64_t ids, cu_seqlens;
+} asap_balance_t;
+uint64_t asap_balance_ws_bytes(int32_t seqs, int32_t e);
+int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream);
+int asap_balance_backward(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t grad_loss,
+                          uint64_t grad_logits, void* stream);
+
+/* counts int32 [e]: how often each expert occurs in ids int32 [t, k] (others are skipped). */
+int asap_expert_counts(uint64_t ids, int32_t t, int32_t k, int32_t e, uint64_t counts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

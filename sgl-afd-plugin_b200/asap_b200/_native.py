@@ -58,6 +58,19 @@ class Fp8Linear_t(ctypes.Structure):
                 ("pad", c_int32)]
 
 
+class Route_t(ctypes.Structure):
+    _fields_ = [("logits", c_uint64), ("ld", c_int64), ("dtype", c_int32), ("t", c_int32), ("e", c_int32),
+                ("k", c_int32), ("sigmoid", c_int32), ("groups", c_int32), ("top_groups", c_int32),
+                ("renormalize", c_int32), ("scale", c_float), ("pad", c_int32), ("bias", c_uint64),
+                ("num_tokens", c_uint64)]
+
+
+class Balance_t(ctypes.Structure):
+    _fields_ = [("logits", c_uint64), ("ld", c_int64), ("dtype", c_int32), ("t", c_int32), ("e", c_int32),
+                ("k", c_int32), ("sigmoid", c_int32), ("seqs", c_int32), ("coef", c_float), ("pad", c_int32),
+                ("ids", c_uint64), ("cu_seqlens", c_uint64)]
+
+
 # name -> (restype, argtypes); every int-returning call is checked
 _SIGS = {
     "asap_last_error_string": (c_char_p, []),
@@ -132,6 +145,12 @@ _SIGS = {
     "asap_fp8_linear_ws_bytes": (c_uint64, [c_int32, c_int32]),
     "asap_fp8_linear": (c_int32, [c_uint64, c_uint64, c_int64, c_int32, c_int32, c_uint64, c_uint64, c_uint64, c_uint64,
                                   c_uint64, c_void_p]),
+    "asap_route": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_void_p]),
+    "asap_route_backward": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_uint64, c_void_p]),
+    "asap_balance_ws_bytes": (c_uint64, [c_int32, c_int32]),
+    "asap_balance_loss": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_void_p]),
+    "asap_balance_backward": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_uint64, c_void_p]),
+    "asap_expert_counts": (c_int32, [c_uint64, c_int32, c_int32, c_int32, c_uint64, c_void_p]),
     "asap_fp8_shared_ws_bytes": (c_uint64, [c_int32, c_int32, c_int32]),
     "asap_fp8_shared": (c_int32, [c_uint64, c_uint64, c_uint64, c_int64, c_int32, c_int32, c_float, c_uint64, c_uint64,
                                   c_uint64, c_uint64, c_uint64, c_void_p]),

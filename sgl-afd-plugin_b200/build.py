@@ -17,7 +17,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "asap_b200", "libasap.so")
-SOURCES = ["transport.cu", "ffn.cu", "linear.cu"]
+SOURCES = ["transport.cu", "ffn.cu", "linear.cu", "router.cu"]
 
 
 def nvcc_path() -> str:

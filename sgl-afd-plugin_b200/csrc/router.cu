@@ -1,0 +1,840 @@
+// libasap router: the top-k choice of an attention rank's MoE layer in the form asap_dispatch takes, its gradient, and
+// the balance loss over the choice with per-expert counts.  The reference takes ids and weights from SGLang's top-k
+// (python/sgl_asap_plugin/srt/layers/moe/ep_moe/layer.py:83-94 receives topk_output).
+//
+// One warp per token; lane l holds experts [l V, l V + V) in registers (V = 1 .. 32, at most 1024 experts), so a row is
+// read once with 16-byte loads and the lowest lane of a tie has the lowest expert.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace asap {
+
+int sm_count();
+
+namespace route {
+
+enum DType { kF32 = 0, kBf16 = 1, kF16 = 2 };
+constexpr int kWarps = 8;  // tokens per block
+
+__device__ __forceinline__ float to_float(uint16_t b, int dt) {
+  if (dt == kBf16) return __uint_as_float((uint32_t)b << 16);
+  return __half2float(__ushort_as_half(b));
+}
+__device__ __forceinline__ float load1(const void* row, int64_t e, int dt) {
+  if (dt == kF32) return reinterpret_cast<const float*>(row)[e];
+  return to_float(reinterpret_cast<const uint16_t*>(row)[e], dt);
+}
+
+// This lane's V values of a row of E; `fill` behind the row's end.  vec: rows start on 16-byte boundaries.
+template <int V>
+__device__ __forceinline__ void load_row(const void* row, int E, int dt, bool vec, int lane, float fill, float (&v)[V]) {
+  const int e0 = lane * V;
+  if (vec && e0 + V <= E) {
+    if (dt == kF32) {
+      const float* p = reinterpret_cast<const float*>(row) + e0;
+      if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(p + i);
+          v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = p[i];
+      }
+    } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + e0;
+      if constexpr (V >= 8) {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p + i);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[i + 2 * j] = to_float((uint16_t)(w[j] & 0xffff), dt);
+            v[i + 2 * j + 1] = to_float((uint16_t)(w[j] >> 16), dt);
+          }
+        }
+      } else if constexpr (V >= 2) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(p + i);
+          v[i] = to_float((uint16_t)(w & 0xffff), dt);
+          v[i + 1] = to_float((uint16_t)(w >> 16), dt);
+        }
+      } else {
+        v[0] = to_float(p[0], dt);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = e0 + i < E ? load1(row, e0 + i, dt) : fill;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dt) {
+  if (dt == kBf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int V>
+__device__ __forceinline__ void store_row(void* row, int E, int dt, bool vec, int lane, const float (&v)[V]) {
+  const int e0 = lane * V;
+  if (vec && e0 + V <= E) {
+    if (dt == kF32) {
+      float* p = reinterpret_cast<float*>(row) + e0;
+      if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+          *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = v[i];
+      }
+      return;
+    }
+    uint16_t* p = reinterpret_cast<uint16_t*>(row) + e0;
+    if constexpr (V >= 8) {
+#pragma unroll
+      for (int i = 0; i < V; i += 8)
+        *reinterpret_cast<uint4*>(p + i) = make_uint4(pack2(v[i], v[i + 1], dt), pack2(v[i + 2], v[i + 3], dt),
+                                                      pack2(v[i + 4], v[i + 5], dt), pack2(v[i + 6], v[i + 7], dt));
+      return;
+    } else if constexpr (V >= 2) {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack2(v[i], v[i + 1], dt);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e0 + i < E) {
+      if (dt == kF32) reinterpret_cast<float*>(row)[e0 + i] = v[i];
+      else reinterpret_cast<uint16_t*>(row)[e0 + i] = (uint16_t)(pack2(v[i], 0.f, dt) & 0xffff);
+    }
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// Order-preserving unsigned keys (0 is free for "closed"; -0 and +0 share one key).
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+  return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+template <typename K>
+__device__ __forceinline__ void top2(K& a, K& b, K x) {
+  if (x > a) {
+    b = a;
+    a = x;
+  } else if (x > b) {
+    b = x;
+  }
+}
+
+struct Args {
+  const void* logits;
+  int64_t ld;
+  int32_t dtype, t, e, k, sigmoid, groups, top_groups, renorm, vec;
+  float scale;
+  const float* bias;         // NULL: none
+  const int32_t* num_tokens;  // NULL: t
+  int32_t* ids;
+  float* weights;
+};
+
+// The k best open keys of the warp's row, best first, ties to the lowest expert: lane j gets the j-th expert's id or -1.
+// With groups, only experts of the top_groups best groups take part; a group counts its best key, or with `pairs` the
+// sum of its two best values (one value if it has one).  tol > 0: returns true when two values that had to be compared
+// lie within tol * (1 + |value|) of each other, so the order may differ from that of unrounded scores.
+template <int V, typename S, typename K>
+__device__ __forceinline__ bool select(const Args& p, const K (&key)[V], uint32_t open, bool pairs, S tol, int lane,
+                                       int& my_id) {
+  bool close = false;
+  if (p.groups > 1) {
+    const int size = p.e / p.groups, lanes = size / V;
+    K best = 0, second = 0, score = 0;
+    if (size % V == 0 && (lanes & (lanes - 1)) == 0) {  // a group is an aligned run of lanes
+#pragma unroll
+      for (int i = 0; i < V; ++i) top2(best, second, (open >> i) & 1u ? key[i] : (K)0);
+      for (int o = 1; o < lanes; o <<= 1) {
+        const K ob = __shfl_xor_sync(0xffffffffu, best, o), os = __shfl_xor_sync(0xffffffffu, second, o);
+        top2(best, second, ob);
+        top2(best, second, os);
+      }
+      best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
+      second = __shfl_sync(0xffffffffu, second, lane * lanes);
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        K a = 0, b = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int e = lane * V + i;
+          top2(a, b, ((open >> i) & 1u) && e >= g * size && e < g * size + size ? key[i] : (K)0);
+        }
+        const K m = warp_max(a);
+        const uint32_t holders = __ballot_sync(0xffffffffu, a == m);
+        const K rest = warp_max(a == m && lane == __ffs(holders) - 1 ? b : a);
+        if (lane == g) {
+          best = m;
+          second = rest;
+        }
+      }
+    }
+    if (lane < p.groups && best)
+      score = pairs ? key_of(value_of(best) + (second ? value_of(second) : (S)0)) : best;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const K o = __shfl_sync(0xffffffffu, score, g);
+      rank += o > score || (o == score && g < lane);
+      if (tol > 0 && g != lane && o && score) {
+        const S d = value_of(o) - value_of(score);
+        close |= fabs(d) < tol * ((S)1 + fabs(value_of(o)));
+      }
+    }
+    const uint32_t kept = __ballot_sync(0xffffffffu, lane < p.groups && score && rank < p.top_groups);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane * V + i;
+      if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
+    }
+  }
+  K best = 0;
+  int at = 0;
+  auto rescan = [&] {
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (((open >> i) & 1u) && key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+  };
+  rescan();
+  my_id = -1;
+  K prev = 0;
+  const int rounds = tol > 0 ? p.k + 1 : p.k;  // the last one only compares the (k+1)-th with the k-th
+  for (int j = 0; j < rounds; ++j) {
+    const K m = warp_max(best);
+    if (!m) break;
+    if (tol > 0 && j > 0) close |= value_of(prev) - value_of(m) < tol * ((S)1 + fabs(value_of(m)));
+    const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
+    const int id = __shfl_sync(0xffffffffu, lane * V + at, src);
+    if (lane == j && j < p.k) my_id = id;
+    if (lane == src) {
+      open &= ~(1u << at);
+      rescan();
+    }
+    prev = m;
+  }
+  return __any_sync(0xffffffffu, close);
+}
+
+// Without a bias the scores rank as the logits do, so the selection compares logits, exactly.  With one it compares
+// score + bias: first in fp32; a row with two candidates closer than the fp32 error (a few in 10^5 rows) is ranked again
+// in 64 bits.  The bound: |score| <= 1 carries at most 2 * 10^-6 (exp within 2 ulp, a sum of up to 1024 terms, one
+// division, one sum), twice that between two of them.
+template <int V>
+__global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constant__ Args p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (t >= p.t) return;
+  int32_t* ids = p.ids + t * p.k;
+  float* weights = p.weights + t * p.k;
+  if (p.num_tokens && t >= *p.num_tokens) {
+    if (lane < p.k) {
+      ids[lane] = -1;
+      weights[lane] = 0.f;
+    }
+    return;
+  }
+  const float ninf = __uint_as_float(0xff800000u);
+  const void* row = reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * (p.dtype == kF32 ? 4 : 2);
+  float l[V];
+  load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, l);
+  uint32_t open = 0;
+  bool nan = false;
+  float top = ninf;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    nan |= l[i] != l[i];
+    if (l[i] > ninf) open |= 1u << i;  // false for NaN
+    top = fmaxf(top, l[i]);
+  }
+  nan = __any_sync(0xffffffffu, nan);
+  float z = 1.f;
+  if (!p.sigmoid) {
+    top = warp_max(top);
+    z = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if ((open >> i) & 1u) z += expf(l[i] - top);
+    z = warp_sum(z);
+  }
+  int id;
+  uint32_t key[V];
+  if (!p.bias) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = key_of(l[i]);
+    select<V, float>(p, key, open, false, 0.f, lane, id);
+  } else {
+    float b[V];
+    load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float s = p.sigmoid ? 1.f / (1.f + expf(-l[i])) : expf(l[i] - top) / z;
+      const float x = s + b[i];
+      if (x == ninf) open &= ~(1u << i);
+      key[i] = x != x ? 1u : key_of(x);
+    }
+    if (select<V, float>(p, key, open, true, 4e-6f, lane, id)) {
+      double zd = 0.0;
+      if (!p.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if ((open >> i) & 1u) zd += exp((double)l[i] - (double)top);
+        zd = warp_sum(zd);
+      }
+      uint64_t wide[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double s = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)top) / zd;
+        const double x = s + (double)b[i];
+        wide[i] = x != x ? 1ull : key_of(x);
+      }
+      select<V, double>(p, wide, open, true, 0.0, lane, id);
+    }
+  }
+  float s = 0.f;
+  if (id >= 0) {
+    const float x = load1(row, id, p.dtype);
+    s = p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - top) / z;
+  }
+  const float sum = p.renorm ? warp_sum(s) + 1e-20f : 1.f;
+  if (lane < p.k) {
+    ids[lane] = id;
+    weights[lane] = nan ? __uint_as_float(0x7fc00000u) : p.scale * (s / sum);
+  }
+}
+
+// ------------------------------------------------------------------ gradient of the weights to the logits
+// w_j = c s_j / N with N = sum of the selected s + 1e-20 (1 without renormalisation).  ds_j = c / N (g_j - [renorm]
+// sum_i g_i s_i / N) on the selected experts; sigmoid: dl_j = s_j (1 - s_j) ds_j.  softmax: dl_e = s_e (ds_e - sum_i
+// ds_i s_i) for every e; after renormalisation that sum is c (sum g s) / N (1 - S / N), nothing unless S is of the size
+// of 1e-20, which only a bias can bring about: `dense` asks for the row.
+struct BackArgs {
+  const void* logits;
+  int64_t ld;
+  int32_t dtype, t, e, k, sigmoid, dense, renorm, vec, out_vec;
+  float scale;
+  const int32_t* ids;
+  const float* grad;
+  void* out;  // [t, e] of the logits' type
+};
+
+template <int V>
+__global__ void __launch_bounds__(32 * kWarps) route_back_kernel(const __grid_constant__ BackArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (t >= p.t) return;
+  const int size = p.dtype == kF32 ? 4 : 2;
+  const void* row = reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * size;
+  const float ninf = __uint_as_float(0xff800000u);
+  int id = -1;
+  float g = 0.f, x = ninf;
+  if (lane < p.k) {
+    id = p.ids[t * p.k + lane];
+    if (id < 0 || id >= p.e) id = -1;
+    if (id >= 0) {
+      g = p.grad[t * p.k + lane];
+      x = load1(row, id, p.dtype);
+    }
+  }
+  float s, d[V];
+  if (p.sigmoid) {
+    s = id >= 0 ? 1.f / (1.f + expf(-x)) : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = 0.f;
+  } else {
+    float z = 0.f, top;
+    if (p.dense) {
+      load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, d);
+      top = ninf;
+#pragma unroll
+      for (int i = 0; i < V; ++i) top = fmaxf(top, d[i]);
+      top = warp_max(top);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        d[i] = d[i] == ninf ? 0.f : expf(d[i] - top);
+        z += d[i];
+      }
+      z = warp_sum(z);
+      z = z > 0.f ? 1.f / z : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] *= z;
+      s = id >= 0 ? expf(x - top) * z : 0.f;
+    } else {  // relative to the selected experts: the common factor cancels
+      top = warp_max(x);
+      s = id >= 0 ? expf(x - top) : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = 0.f;
+    }
+  }
+  const float n = p.renorm ? warp_sum(s) + (p.sigmoid || p.dense ? 1e-20f : 0.f) : 1.f;
+  const float gs = p.renorm ? warp_sum(g * s) / n : 0.f;
+  float ds = id >= 0 ? p.scale / n * (g - gs) : 0.f;
+  float mine;  // this lane's selected expert: its gradient beyond the dense term
+  if (p.sigmoid) {
+    mine = id >= 0 ? ds * s * (1.f / (1.f + expf(x))) : 0.f;  // 1 - s without cancellation
+  } else {
+    const float dot = p.dense ? warp_sum(ds * s) : 0.f;
+    mine = ds * s;
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = p.dense ? -d[i] * dot : 0.f;
+  }
+  for (int j = 0; j < p.k; ++j) {
+    const int e = __shfl_sync(0xffffffffu, id, j);
+    const float v = __shfl_sync(0xffffffffu, mine, j);
+    if (e >= 0 && e / V == lane) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (e % V == i) d[i] += v;
+    }
+  }
+  store_row<V>(reinterpret_cast<uint8_t*>(p.out) + t * p.e * size, p.e, p.dtype, p.out_vec, lane, d);
+}
+
+// ------------------------------------------------------------------ balance loss
+// Over the sequences s with n_s > 0 live tokens (a token is live when it has an id), S' of them:
+//   L = coef / S' sum_s sum_e f_se P_se,  f_se = E / (k n_s) c_se,  P_se = 1 / n_s sum_t p_te,
+// c the counts, p the row's softmax, or its sigmoids normalised to sum 1.  With a_se = coef / S' E / (k n_s^2) c_se that
+// is a plain sum over tokens, L = sum_t sum_e a_se p_te, and the gradient is dl_te = p_te (a_se - sum_i a_si p_ti),
+// times 1 - sigmoid(l_te) for sigmoids: once the counts are there, each direction is one pass over the rows, and no sum
+// of probabilities over tokens is kept.
+struct BalanceArgs {
+  const void* logits;
+  int64_t ld;
+  int32_t dtype, t, e, k, sigmoid, seqs, vec, out_vec;
+  float coef;
+  const int32_t* ids;
+  const int32_t* cu;   // [seqs + 1], NULL: one sequence of t tokens
+  int32_t* counts;     // [seqs, e]
+  int32_t* live;       // [seqs]
+  uint32_t* ticket;
+  double* partial;     // [grid]
+  float* loss;
+  const float* grad;   // d loss, scalar
+  void* out;
+};
+
+// the sequence of token t, or -1 (before the first or behind the last)
+__device__ __forceinline__ int seq_of(const int32_t* cu, int seqs, int64_t t) {
+  if (!cu) return 0;
+  if (t < cu[0]) return -1;
+  int lo = 0, hi = seqs;  // first s with cu[s + 1] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo < seqs ? lo : -1;
+}
+
+constexpr int kCountRows = 128;  // tokens per block, one per thread
+__global__ void __launch_bounds__(kCountRows) balance_count_kernel(const __grid_constant__ BalanceArgs p) {
+  extern __shared__ int32_t hist[];  // the counts of the block's first sequence; [e] = its live tokens
+  for (int i = threadIdx.x; i <= p.e; i += kCountRows) hist[i] = 0;
+  const int64_t t0 = (int64_t)blockIdx.x * kCountRows, t = t0 + threadIdx.x;
+  const int first = seq_of(p.cu, p.seqs, t0);
+  __syncthreads();
+  const int s = t < p.t ? seq_of(p.cu, p.seqs, t) : -1;
+  if (s >= 0) {
+    const int32_t* ids = p.ids + t * p.k;
+    bool any = false;
+    for (int j = 0; j < p.k; ++j) {
+      const int e = ids[j];
+      if (e < 0 || e >= p.e) continue;
+      any = true;
+      atomicAdd(s == first ? &hist[e] : &p.counts[(int64_t)s * p.e + e], 1);
+    }
+    if (any && p.live) atomicAdd(s == first ? &hist[p.e] : &p.live[s], 1);
+  }
+  __syncthreads();
+  if (first < 0) return;
+  for (int i = threadIdx.x; i <= p.e; i += kCountRows)
+    if (hist[i]) {
+      if (i < p.e) atomicAdd(&p.counts[(int64_t)first * p.e + i], hist[i]);
+      else if (p.live) atomicAdd(&p.live[first], hist[i]);
+    }
+}
+
+// p_e of a row.  With sigmoids a row whose largest logit is negative is scaled by e^-top, so that its values do not
+// underflow before they are normalised.
+template <int V>
+__device__ __forceinline__ void row_probabilities(bool sigmoid, float (&l)[V], float (&p)[V]) {
+  const float ninf = __uint_as_float(0xff800000u);
+  float top = ninf, z = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+  top = warp_max(top);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (l[i] == ninf) p[i] = 0.f;
+    else if (!sigmoid) p[i] = expf(l[i] - top);
+    else if (top >= 0.f) p[i] = 1.f / (1.f + expf(-l[i]));
+    else p[i] = expf(l[i] - top) / (1.f + expf(l[i]));
+    z += p[i];
+  }
+  z = warp_sum(z);
+  const float r = z > 0.f ? 1.f / z : (z != z ? z : 0.f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) p[i] *= r;
+}
+
+template <int V, bool BACK>
+__global__ void __launch_bounds__(32 * kWarps) balance_kernel(const __grid_constant__ BalanceArgs p) {
+  __shared__ int s_filled[kWarps];
+  __shared__ double s_sum[kWarps];
+  __shared__ bool s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int filled = 0;
+  for (int s = threadIdx.x; s < p.seqs; s += 32 * kWarps) filled += p.live[s] > 0;
+  filled = __reduce_add_sync(0xffffffffu, filled);
+  if (lane == 0) s_filled[warp] = filled;
+  __syncthreads();
+  filled = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) filled += s_filled[w];
+  const float base = p.coef / (float)max(filled, 1) * ((float)p.e / (float)p.k) * (BACK ? *p.grad : 1.f);
+  const int size = p.dtype == kF32 ? 4 : 2;
+  const float ninf = __uint_as_float(0xff800000u);
+  double sum = 0.0;
+  for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < p.t; t += (int64_t)gridDim.x * kWarps) {
+    const int s = seq_of(p.cu, p.seqs, t);
+    const int id = lane < p.k ? p.ids[t * p.k + lane] : -1;
+    const bool live = __any_sync(0xffffffffu, id >= 0 && id < p.e) && s >= 0;
+    float d[V];
+    if (live) {
+      float l[V], pr[V];
+      load_row<V>(reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * size, p.e, p.dtype, p.vec, lane, ninf, l);
+      row_probabilities<V>(p.sigmoid != 0, l, pr);
+      const float n = (float)p.live[s];
+      const float a = base / (n * n);
+      const int32_t* counts = p.counts + (int64_t)s * p.e + lane * V;
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        d[i] = lane * V + i < p.e ? a * (float)counts[i] : 0.f;
+        dot += d[i] * pr[i];
+      }
+      dot = warp_sum(dot);
+      if constexpr (BACK) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          d[i] = pr[i] * (d[i] - dot);
+          if (p.sigmoid) d[i] *= 1.f / (1.f + expf(l[i]));
+        }
+      } else {
+        sum += (double)dot;
+      }
+    } else if constexpr (BACK) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = 0.f;
+    }
+    if constexpr (BACK)
+      store_row<V>(reinterpret_cast<uint8_t*>(p.out) + t * p.e * size, p.e, p.dtype, p.out_vec, lane, d);
+  }
+  if constexpr (!BACK) {
+    // block sums, added in block order by the block that finishes last: the same bits every time
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double b = 0.0;
+      for (int w = 0; w < kWarps; ++w) b += s_sum[w];
+      p.partial[blockIdx.x] = b;
+      __threadfence();
+      s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (s_last && warp == 0) {
+      __threadfence();
+      double b = 0.0;
+      for (int i = lane; i < (int)gridDim.x; i += 32) b += __ldcg(&p.partial[i]);
+      b = warp_sum(b);
+      if (lane == 0) *p.loss = (float)b;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+template <template <int> class F, typename A>
+static void by_experts(int e, const A& a, int grid, cudaStream_t st) {
+  if (e <= 32) F<1>::run(a, grid, st);
+  else if (e <= 64) F<2>::run(a, grid, st);
+  else if (e <= 128) F<4>::run(a, grid, st);
+  else if (e <= 256) F<8>::run(a, grid, st);
+  else if (e <= 512) F<16>::run(a, grid, st);
+  else F<32>::run(a, grid, st);
+}
+template <int V>
+struct Forward {
+  static void run(const Args& a, int grid, cudaStream_t st) { route_kernel<V><<<grid, 32 * kWarps, 0, st>>>(a); }
+};
+template <int V>
+struct Backward {
+  static void run(const BackArgs& a, int grid, cudaStream_t st) { route_back_kernel<V><<<grid, 32 * kWarps, 0, st>>>(a); }
+};
+template <int V>
+struct Loss {
+  static void run(const BalanceArgs& a, int grid, cudaStream_t st) {
+    balance_kernel<V, false><<<grid, 32 * kWarps, 0, st>>>(a);
+  }
+};
+template <int V>
+struct LossBack {
+  static void run(const BalanceArgs& a, int grid, cudaStream_t st) {
+    balance_kernel<V, true><<<grid, 32 * kWarps, 0, st>>>(a);
+  }
+};
+
+static int check_logits(const char* fn, uint64_t logits, int64_t ld, int32_t dtype, int32_t t, int32_t e, int32_t k) {
+  if (t < 1 || e < 1 || e > ASAP_ROUTE_MAX_EXPERTS || k < 1 || k > ASAP_ROUTE_MAX_TOPK || k > e || t > (1 << 24)) {
+    set_error("%s: need 1 to %d tokens, 1 <= k <= %d, k <= experts <= %d (got %d tokens, k = %d, %d experts)", fn, 1 << 24,
+              ASAP_ROUTE_MAX_TOPK, ASAP_ROUTE_MAX_EXPERTS, t, k, e);
+    return ASAP_EINVAL;
+  }
+  if (dtype < 0 || dtype > 2 || !logits || (logits & (dtype ? 1 : 3)) || ld < e) {
+    set_error("%s: logits must be fp32 (0), bf16 (1) or fp16 (2), aligned to their type, with a row stride of at least "
+              "%d (got type %d, stride %lld)", fn, e, dtype, (long long)ld);
+    return ASAP_EINVAL;
+  }
+  return ASAP_OK;
+}
+static bool rows_16(uint64_t base, int64_t ld, int32_t dtype) {
+  return (base & 15) == 0 && (ld * (dtype ? 2 : 4)) % 16 == 0;
+}
+
+struct BalanceWs {
+  uint64_t live, ticket, partial, zeroed, bytes;
+};
+static BalanceWs balance_ws(int64_t seqs, int64_t e) {
+  BalanceWs w;
+  w.live = 4 * seqs * e;
+  w.ticket = w.live + 4 * seqs;
+  w.zeroed = w.ticket + 4;
+  w.partial = align_up(w.zeroed, 8);
+  w.bytes = w.partial + 8ull * 8 * sm_count();
+  return w;
+}
+static int balance_grid(int32_t t) {
+  const int64_t blocks = ((int64_t)t + kWarps - 1) / kWarps, cap = 8ll * sm_count();
+  return (int)(blocks < cap ? blocks : cap);
+}
+
+static int balance_args(const char* fn, BalanceArgs& a, const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes) {
+  if (!b) {
+    set_error("%s: NULL argument", fn);
+    return ASAP_EINVAL;
+  }
+  if (int rc = check_logits(fn, b->logits, b->ld, b->dtype, b->t, b->e, b->k)) return rc;
+  if (!b->ids || (b->ids & 3) || b->seqs < 1 || b->seqs > (1 << 20) || (!b->cu_seqlens && b->seqs != 1) ||
+      (b->cu_seqlens & 3)) {
+    set_error("%s: need ids and 1 to %d sequences (one without offsets), got %d", fn, 1 << 20, b->seqs);
+    return ASAP_EINVAL;
+  }
+  const BalanceWs w = balance_ws(b->seqs, b->e);
+  if (!ws || (ws & 7) || ws_bytes < w.bytes) {
+    set_error("%s: the workspace must be 8-byte aligned and hold %llu bytes (got %llu)", fn, (unsigned long long)w.bytes,
+              (unsigned long long)ws_bytes);
+    return ASAP_EINVAL;
+  }
+  a.logits = (const void*)b->logits;
+  a.ld = b->ld;
+  a.dtype = b->dtype;
+  a.t = b->t;
+  a.e = b->e;
+  a.k = b->k;
+  a.sigmoid = b->sigmoid;
+  a.seqs = b->seqs;
+  a.vec = rows_16(b->logits, b->ld, b->dtype);
+  a.coef = b->coef;
+  a.ids = (const int32_t*)b->ids;
+  a.cu = (const int32_t*)b->cu_seqlens;
+  a.counts = (int32_t*)ws;
+  a.live = (int32_t*)(ws + w.live);
+  a.ticket = (uint32_t*)(ws + w.ticket);
+  a.partial = (double*)(ws + w.partial);
+  return ASAP_OK;
+}
+
+}  // namespace route
+}  // namespace asap
+
+using namespace asap;
+
+extern "C" {
+
+int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stream) {
+  if (!r) {
+    set_error("asap_route: NULL argument");
+    return ASAP_EINVAL;
+  }
+  if (int rc = route::check_logits("asap_route", r->logits, r->ld, r->dtype, r->t, r->e, r->k)) return rc;
+  if (r->groups < 1 || r->groups > 32 || r->e % r->groups || r->top_groups < 1 || r->top_groups > r->groups) {
+    set_error("asap_route: %d groups of %d experts, %d kept: need 1 to 32 equal groups and 1 <= kept <= groups",
+              r->groups, r->e, r->top_groups);
+    return ASAP_EINVAL;
+  }
+  if (!ids || (ids & 3) || !weights || (weights & 3) || (r->bias & 3) || (r->num_tokens & 3)) {
+    set_error("asap_route: ids and weights must be non-NULL, and every pointer 4-byte aligned");
+    return ASAP_EINVAL;
+  }
+  route::Args a{};
+  a.logits = (const void*)r->logits;
+  a.ld = r->ld;
+  a.dtype = r->dtype;
+  a.t = r->t;
+  a.e = r->e;
+  a.k = r->k;
+  a.sigmoid = r->sigmoid;
+  a.groups = r->top_groups == r->groups ? 1 : r->groups;  // every group kept: no limit
+  a.top_groups = r->top_groups;
+  a.renorm = r->renormalize;
+  a.vec = route::rows_16(r->logits, r->ld, r->dtype);
+  a.scale = r->scale;
+  a.bias = (const float*)r->bias;
+  a.num_tokens = (const int32_t*)r->num_tokens;
+  a.ids = (int32_t*)ids;
+  a.weights = (float*)weights;
+  route::by_experts<route::Forward>(r->e, a, (r->t + route::kWarps - 1) / route::kWarps, (cudaStream_t)stream);
+  ASAP_CHECK_LAUNCH("route_kernel");
+  return ASAP_OK;
+}
+
+int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weights, uint64_t grad_logits,
+                        void* stream) {
+  if (!r) {
+    set_error("asap_route_backward: NULL argument");
+    return ASAP_EINVAL;
+  }
+  if (int rc = route::check_logits("asap_route_backward", r->logits, r->ld, r->dtype, r->t, r->e, r->k)) return rc;
+  if (!ids || (ids & 3) || !grad_weights || (grad_weights & 3) || !grad_logits || (grad_logits & 3)) {
+    set_error("asap_route_backward: ids, grad_weights and grad_logits must be non-NULL and 4-byte aligned");
+    return ASAP_EINVAL;
+  }
+  route::BackArgs a{};
+  a.logits = (const void*)r->logits;
+  a.ld = r->ld;
+  a.dtype = r->dtype;
+  a.t = r->t;
+  a.e = r->e;
+  a.k = r->k;
+  a.sigmoid = r->sigmoid;
+  a.renorm = r->renormalize;
+  a.dense = !r->sigmoid && (!r->renormalize || r->bias);
+  a.vec = route::rows_16(r->logits, r->ld, r->dtype);
+  a.out_vec = route::rows_16(grad_logits, r->e, r->dtype);
+  a.scale = r->scale;
+  a.ids = (const int32_t*)ids;
+  a.grad = (const float*)grad_weights;
+  a.out = (void*)grad_logits;
+  route::by_experts<route::Backward>(r->e, a, (r->t + route::kWarps - 1) / route::kWarps, (cudaStream_t)stream);
+  ASAP_CHECK_LAUNCH("route_back_kernel");
+  return ASAP_OK;
+}
+
+uint64_t asap_balance_ws_bytes(int32_t seqs, int32_t e) {
+  if (seqs < 1 || seqs > (1 << 20) || e < 1 || e > ASAP_ROUTE_MAX_EXPERTS) return 0;
+  return route::balance_ws(seqs, e).bytes;
+}
+
+int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream) {
+  route::BalanceArgs a{};
+  if (int rc = route::balance_args("asap_balance_loss", a, b, ws, ws_bytes)) return rc;
+  if (!loss || (loss & 3)) {
+    set_error("asap_balance_loss: loss must be non-NULL and 4-byte aligned");
+    return ASAP_EINVAL;
+  }
+  a.loss = (float*)loss;
+  cudaStream_t st = (cudaStream_t)stream;
+  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->seqs, b->e).zeroed, st));
+  route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountRows, 4 * (b->e + 1),
+                                st>>>(a);
+  ASAP_CHECK_LAUNCH("balance_count_kernel");
+  route::by_experts<route::Loss>(b->e, a, route::balance_grid(b->t), st);
+  ASAP_CHECK_LAUNCH("balance_kernel");
+  return ASAP_OK;
+}
+
+int asap_balance_backward(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t grad_loss,
+                          uint64_t grad_logits, void* stream) {
+  route::BalanceArgs a{};
+  if (int rc = route::balance_args("asap_balance_backward", a, b, ws, ws_bytes)) return rc;
+  if (!grad_loss || (grad_loss & 3) || !grad_logits || (grad_logits & 3)) {
+    set_error("asap_balance_backward: grad_loss and grad_logits must be non-NULL and 4-byte aligned");
+    return ASAP_EINVAL;
+  }
+  a.grad = (const float*)grad_loss;
+  a.out = (void*)grad_logits;
+  a.out_vec = route::rows_16(grad_logits, b->e, b->dtype);
+  route::by_experts<route::LossBack>(b->e, a, route::balance_grid(b->t), (cudaStream_t)stream);
+  ASAP_CHECK_LAUNCH("balance_kernel (gradient)");
+  return ASAP_OK;
+}
+
+int asap_expert_counts(uint64_t ids, int32_t t, int32_t k, int32_t e, uint64_t counts, void* stream) {
+  if (!ids || (ids & 3) || !counts || (counts & 3) || t < 1 || t > (1 << 24) || k < 1 || k > ASAP_ROUTE_MAX_TOPK ||
+      e < 1 || e > ASAP_ROUTE_MAX_EXPERTS) {
+    set_error("asap_expert_counts: need ids and counts (4-byte aligned), 1 to %d tokens, k <= %d, 1 to %d experts (got "
+              "%d, %d, %d)", 1 << 24, ASAP_ROUTE_MAX_TOPK, ASAP_ROUTE_MAX_EXPERTS, t, k, e);
+    return ASAP_EINVAL;
+  }
+  route::BalanceArgs a{};
+  a.t = t;
+  a.e = e;
+  a.k = k;
+  a.seqs = 1;
+  a.ids = (const int32_t*)ids;
+  a.counts = (int32_t*)counts;
+  cudaStream_t st = (cudaStream_t)stream;
+  ASAP_CUDA(cudaMemsetAsync((void*)counts, 0, 4ull * e, st));
+  route::balance_count_kernel<<<(t + route::kCountRows - 1) / route::kCountRows, route::kCountRows, 4 * (e + 1), st>>>(a);
+  ASAP_CHECK_LAUNCH("balance_count_kernel");
+  return ASAP_OK;
+}
+
+}  // extern "C"
