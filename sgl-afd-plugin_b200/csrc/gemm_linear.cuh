@@ -208,7 +208,6 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           }
           mbar_wait(&full[s], ph, drain_deadline, &no_abort);
         }
-        if (!ok) report(p.status, status_word(ASAP_ST_PIPELINE_TIMEOUT, 0, 0, 16 + SWIGLU));
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer: one K block per TMEM buffer, alternating
@@ -371,6 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) report(p.status, status_word(ASAP_ST_PIPELINE_TIMEOUT, 0, 0, 16 + SWIGLU));
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);

@@ -20,6 +20,7 @@ int sm_count();
 namespace lin {
 
 constexpr float kE4M3Max = 448.f;
+constexpr int kMaxSmem = 232448;  // shared memory a block may have
 
 // Scale of one block of activations and the factor that maps it to the code range.  The absolute maximum counts as at
 // least 1e-10, so a block of zeros has codes 0.  pow2: amax / 448 rounded up to a power of two, by its bits (448 =
@@ -42,6 +43,24 @@ __device__ __forceinline__ uint32_t codes4(const float* v, float inv) {
   return cvt_e4m3x2(v[0] * inv, v[1] * inv) | (cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16);
 }
 
+// A half-warp's block of 128 16-bit values, 8 per lane -> this lane's 8 codes, and the block's scale
+__device__ __forceinline__ void quant8(const uint4& u, bool fp16, bool pow2, uint2& codes, float& scale) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  float v[8], amax = 0.f, inv;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                          : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  block_scale(amax, pow2, scale, inv);
+  codes = make_uint2(codes4(v, inv), codes4(v + 4, inv));
+}
+
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
   if (limit > 0.f) {
     g = fminf(g, limit);
@@ -53,6 +72,7 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 }  // namespace lin
 
 #include "gemm_linear.cuh"
+#include "gemm_skinny.cuh"
 
 namespace lin {
 
@@ -75,25 +95,13 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const __grid_constant__
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < items; i += step) {
     const int64_t row = i / chunks;
     const int col = (int)(i - row * chunks) * 256 + lane * 8;
-    float v[8];
     uint4 u = make_uint4(0, 0, 0, 0);
     if (col < p.K) u = *reinterpret_cast<const uint4*>(p.x + row * p.ldx + col);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float amax = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = p.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
-                              : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-      amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float scale, inv;
-    block_scale(amax, p.pow2 != 0, scale, inv);
+    uint2 codes;
+    float scale;
+    quant8(u, p.fp16 != 0, p.pow2 != 0, codes, scale);
     if (col < p.KB * 128) {
-      *reinterpret_cast<uint2*>(p.xq + row * p.KB * 128 + col) = make_uint2(codes4(v, inv), codes4(v + 4, inv));
+      *reinterpret_cast<uint2*>(p.xq + row * p.KB * 128 + col) = codes;
       if ((lane & 15) == 0) p.sa[(int64_t)(col / 128) * p.mp + row] = scale;
     }
   }
@@ -125,6 +133,11 @@ static int ensure_attrs() {
   if (dev >= 0 && dev < 64 && done[dev]) return ASAP_OK;
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  for (const void* f : {(const void*)linear_skinny_kernel<16, 0>, (const void*)linear_skinny_kernel<32, 0>,
+                        (const void*)linear_skinny_kernel<64, 0>, (const void*)linear_skinny_kernel<128, 0>,
+                        (const void*)linear_skinny_kernel<16, 1>, (const void*)linear_skinny_kernel<32, 1>,
+                        (const void*)linear_skinny_kernel<64, 1>})
+    ASAP_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
   if (dev >= 0 && dev < 64) done[dev] = true;
   return ASAP_OK;
 }
@@ -218,6 +231,80 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
   return ASAP_OK;
 }
 
+// ------------------------------------------------------------------ few rows
+// How a product of few rows is launched, or split = 0: not at all.
+struct SkinnyPlan {
+  int tn, split, stages, max_kb, smem;
+};
+
+// TN is the smallest of 16, 32, 64, 128 that holds the rows (64 at most with SwiGLU, whose tiles are two), halved while
+// a CTA's part of x does not fit beside the fewest stages.  K is split as far as the grid stays within two CTAs per SM.
+template <int SWIGLU>
+static SkinnyPlan skinny_plan(const Linear* L, int32_t m) {
+  const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
+  int tn = m <= 16 ? 16 : m <= 32 ? 32 : (m <= 64 || SWIGLU) ? 64 : 128;
+  for (; tn >= 16; tn /= 2) {
+    const int64_t y = (m + tn - 1) / tn;
+    int split = 1;
+    while (split < SK_MAX_SPLIT && 2 * split <= L->KB && n_tiles * y * split * 2 <= 2 * sm_count()) split *= 2;
+    for (; split <= SK_MAX_SPLIT && split <= L->KB; split *= 2) {
+      SkinnyPlan pl;
+      pl.tn = tn;
+      pl.split = split;
+      pl.max_kb = (L->KB + split - 1) / split;
+      const int tiles = SWIGLU ? 2 : 1, stage = tiles * 128 * BK, part = tiles * tn * 512;
+      const int least = part > 3 * stage ? (part + stage - 1) / stage : 3;
+      const int fixed = 1024 + 2048 + pl.max_kb * (tn * BK + tn * 4 + 8);
+      if (pl.max_kb > SK_MAX_KB || fixed + least * stage > kMaxSmem) continue;
+      // half an SM's shared memory if three stages fit it, so that two CTAs share the SM
+      const int half = kMaxSmem / 2 - 1024;
+      const int room = tiles * tn <= 64 && fixed + least * stage <= half ? half : kMaxSmem;
+      pl.stages = (room - fixed) / stage;
+      if (pl.stages > SK_MAX_STAGES) pl.stages = SK_MAX_STAGES;
+      if (pl.stages > pl.max_kb) pl.stages = pl.max_kb;
+      if (pl.stages < least) pl.stages = least;
+      pl.smem = fixed + pl.stages * stage;
+      // never three CTAs on an SM: the third would wait for tensor memory while its cluster waits for it
+      if (pl.smem < 80 * 1024) pl.smem = 80 * 1024;
+      return pl;
+    }
+  }
+  return SkinnyPlan{0, 0, 0, 0, 0};
+}
+
+template <int SWIGLU>
+static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, cudaStream_t st) {
+  p.tmap_w = L->map;
+  p.K = L->d.k;
+  p.N = L->d.n;
+  p.KB = L->KB;
+  p.NB = L->NB;
+  p.split = pl.split;
+  p.stages = pl.stages;
+  p.max_kb = pl.max_kb;
+  p.sb = (const float*)L->d.scale;
+  p.pow2 = L->d.pow2;
+  const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n_tiles * pl.split, (p.M + pl.tn - 1) / pl.tn);
+  cfg.blockDim = dim3(SK_THREADS);
+  cfg.dynamicSmemBytes = pl.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = pl.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (pl.tn == 16) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<16, SWIGLU>, p));
+  else if (pl.tn == 32) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<32, SWIGLU>, p));
+  else if (pl.tn == 64) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<64, SWIGLU>, p));
+  else if constexpr (!SWIGLU) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<128, 0>, p));
+  return ASAP_OK;
+}
+
+constexpr int kSkinnyRows = 64;  // at most this many rows take the few-rows kernel
+
 }  // namespace lin
 }  // namespace asap
 
@@ -293,6 +380,20 @@ int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t
   if (int rc = lin::check_rows("asap_fp8_linear", m, x, ldx, L->d.k, out, ws, ws_bytes, need)) return rc;
   if (int rc = lin::ensure_attrs()) return rc;
   cudaStream_t st = (cudaStream_t)stream;
+  if (m <= lin::kSkinnyRows) {
+    const lin::SkinnyPlan pl = lin::skinny_plan<0>(L, m);
+    if (pl.split) {
+      lin::SkinnyParams p{};
+      p.x = (const uint16_t*)x;
+      p.ldx = ldx;
+      p.M = m;
+      p.fp16 = fp16;
+      p.out = (void*)out;
+      p.status = status;
+      p.timeout_ns = timeout_ns;
+      return lin::skinny<0>(L, pl, p, st);
+    }
+  }
   const lin::ActWs a = lin::act_ws(m, L->d.k);
   if (int rc = lin::quantise(x, ldx, m, L, fp16, ws, ws + a.codes, a.mp, st)) return rc;
   return lin::product(L, false, ws, ws + a.codes, m, a.mp, out, L->d.n, fp16, 0.f, 0, 0, status, timeout_ns, st);
@@ -324,6 +425,28 @@ int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t
   cudaStream_t st = (cudaStream_t)stream;
   const lin::ActWs a = lin::act_ws(m, H), b = lin::act_ws(m, I);
   const uint64_t sa = ws + a.codes, hq = sa + a.scales, sh = hq + b.codes;
+  if (m <= lin::kSkinnyRows) {
+    const lin::SkinnyPlan up = lin::skinny_plan<1>(L13, m), down = lin::skinny_plan<0>(L2, m);
+    if (up.split && down.split) {
+      lin::SkinnyParams p{};
+      p.x = (const uint16_t*)x;
+      p.ldx = ldx;
+      p.M = m;
+      p.fp16 = fp16;
+      p.swiglu_limit = swiglu_limit;
+      p.out_q = (uint8_t*)hq;
+      p.out_sa = (float*)sh;
+      p.mp = b.mp;
+      p.status = status;
+      p.timeout_ns = timeout_ns;
+      if (int rc = lin::skinny<1>(L13, up, p, st)) return rc;
+      p.x = nullptr;
+      p.xq = (const uint8_t*)hq;
+      p.sa = (const float*)sh;
+      p.out = (void*)out;
+      return lin::skinny<0>(L2, down, p, st);
+    }
+  }
   if (int rc = lin::quantise(x, ldx, m, L13, fp16, ws, sa, a.mp, st)) return rc;
   if (int rc = lin::product(L13, true, ws, sa, m, a.mp, 0, 0, fp16, swiglu_limit, hq, sh, status, timeout_ns, st))
     return rc;
