@@ -5,10 +5,14 @@
 // of two and cannot ride in the MMA, so every 128-deep K block is accumulated on its own into one of two TMEM buffers
 // and folded into fp32 registers (one fma per element) while the tensor core fills the other buffer.
 //
-// A probe of the fold alone (148 SMs, operands fixed in shared memory) runs one K block of 128 x 256 in 390 cycles,
-// and with the MMAs and their hand-over in 640, against 512 for the MMAs by themselves.  What keeps a kernel from
-// that is a global load on the fold's path: so one warp multiplies the two scales of each row and K block ahead of
-// time into a ring of shared-memory slots (kScaleSlots K blocks, about 4 K cycles, deep) and the fold reads one word.
+// What bounds it is the turn-around of those two buffers: MMA done -> a folding warp sees it -> two TMEM loads, half
+// the fmas, two more loads -> the MMA issuer sees the buffer free.  A wait on an mbarrier costs about 200 cycles here
+// even when its phase is long over (the MMAs keep shared memory busy), and the issuer used to make three per K block,
+// which alone took 620 of its 1170 cycles.  So a K block has one barrier to start (`ready`: operands and scales
+// landed, buffer free) and one when it is done (`done`: stage free, partial complete).  The activation scales come
+// through the same ring, a K block ahead of the operands (512 bytes per block): when a block is done the next one's
+// scales have landed, and a folding warp reads them while its last fmas run, so that neither a load from memory nor one
+// from shared memory (200 cycles as well) is on the turn-around.
 #pragma once
 
 namespace lin {
@@ -16,15 +20,19 @@ namespace lin {
 constexpr int BM = 128, BN = 256, BK = 128;
 constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, B_HALF = B_BYTES / 2;
+constexpr int SCALE_BYTES = BM * 4;  // a K block's activation scales
+// Slots of scales: the copy for K block it + SCALE_SLOTS is issued with the operands of the block before it, after
+// done(it + SCALE_SLOTS - 1 - STAGES), whose MMAs waited for every folding warp to be through with K block
+// it + SCALE_SLOTS - 3 - STAGES >= it.
+constexpr int SCALE_SLOTS = 8;
+static_assert(SCALE_SLOTS >= STAGES + 3, "a folding warp may still read the slot");
 constexpr uint32_t STAGE_TX = A_BYTES + B_BYTES;
-constexpr int kScaleSlots = 8;
-constexpr int SCALE_BYTES = 2 * BM * 4;  // a K block's factor per row, one set per 128 weight rows of the tile
 constexpr int EPI_WARPS = 8, EPI_BASE = 4, THREADS = 32 * (EPI_BASE + EPI_WARPS);
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int STAGE_OUT_BYTES = EPI_WARPS * 2048;
 constexpr int CTRL_BYTES = 4096;  // barriers, TMEM slot, row amax exchange
 constexpr int SMEM_BYTES =
-    1024 + STAGES * (A_BYTES + B_BYTES) + kScaleSlots * SCALE_BYTES + STAGE_OUT_BYTES + CTRL_BYTES;
+    1024 + STAGES * (A_BYTES + B_BYTES) + SCALE_SLOTS * SCALE_BYTES + STAGE_OUT_BYTES + CTRL_BYTES;
 static_assert(SMEM_BYTES <= 232448, "shared memory over the 227 KB per block");
 // m-tiles that share a pass over the weight tiles: 16 x 9 tiles are in flight on 148 SMs, so a K block of both
 // operands is read from L2 about 12 times per 128-row tile whatever M and N are.
@@ -56,21 +64,57 @@ __device__ __forceinline__ uint64_t sdesc_sw128(const void* p) {
   return ((a >> 4) & 0x3FFFull) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// A bounded wait of a whole warp: every lane gets the same answer and the warp is converged after it.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t deadline, volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline, abort));
+// A bounded wait of a whole warp: one lane polls, every lane gets its answer and the warp is converged after it.  (With
+// 32 lanes polling, the folding and scale warps filled the shared-memory pipe: a wait on a barrier that had long
+// completed then took the MMA issuer 210 cycles, three of them per K block.)  It ends when another warp's wait has run
+// out (the producer and the MMA issuer watch the clock) or after kSpins tries, some seconds: a count is an immediate, a
+// deadline would hold two registers that the folding warps do not have.
+constexpr uint32_t kSpins = 1u << 27;
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) {
+    for (uint32_t it = 0; ok && !mbar_try_wait(bar, parity);) {
+      ++it;
+      if ((it & 255u) == 0 && (*abort || it > kSpins)) {
+        *abort = 1;
+        ok = 0;
+      }
+    }
+  }
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-// acc[i] += x[i] * f, two per instruction
-__device__ __forceinline__ void fold32(float* acc, const uint32_t (&x)[32], float f) {
-  const float2 ff = make_float2(f, f);
+// tcgen05.wait::ld that the uses of `r` cannot be moved above
+__device__ __forceinline__ void tmem_wait_regs(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// acc[2i], acc[2i + 1] += x[2i], x[2i + 1] times f: the packed fp32 fma, each half one fused multiply-add with one
+// rounding.  volatile keeps them between the TMEM loads they are written between; left to the compiler's order, a K
+// block took 1650 cycles instead of 900.
+__device__ __forceinline__ void fold32(uint64_t* acc, const uint32_t (&x)[32], uint64_t ff) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 r = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), ff,
-                                make_float2(acc[2 * i], acc[2 * i + 1]));
-    acc[2 * i] = r.x;
-    acc[2 * i + 1] = r.y;
-  }
+  for (int i = 0; i < 16; ++i)
+    asm volatile("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}"
+                 : "+l"(acc[i])
+                 : "r"(x[2 * i]), "r"(x[2 * i + 1]), "l"(ff));
+}
+__device__ __forceinline__ uint64_t twice(float f) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(f));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
 }
 
 __device__ __forceinline__ void decode_tile(const Params& p, int tile, int& m_t, int& n_t) {
@@ -116,16 +160,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + STAGES * A_BYTES;
-  float* sF = reinterpret_cast<float*>(sB + STAGES * B_BYTES);  // [kScaleSlots][2][BM]
-  uint8_t* sOut = reinterpret_cast<uint8_t*>(sF) + kScaleSlots * SCALE_BYTES;
+  float* sSa = reinterpret_cast<float*>(sB + STAGES * B_BYTES);  // [SCALE_SLOTS][BM]
+  uint8_t* sOut = reinterpret_cast<uint8_t*>(sSa) + SCALE_SLOTS * SCALE_BYTES;
   uint8_t* ctrl = sOut + STAGE_OUT_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ctrl);
-  uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;         // [2]
-  uint64_t* acc_empty = acc_full + 2;          // [2]
-  uint64_t* sc_full = acc_empty + 2;           // [kScaleSlots]
-  uint64_t* sc_empty = sc_full + kScaleSlots;  // [kScaleSlots]
-  uint64_t* mma_done = sc_empty + kScaleSlots;
+  // K block `it` uses stage it % STAGES, scale slot it % SCALE_SLOTS and TMEM buffer it % 2
+  uint64_t* ready = reinterpret_cast<uint64_t*>(ctrl);  // [STAGES] operands, scales and buffer: the MMAs may start
+  uint64_t* done = ready + STAGES;                      // [STAGES] the MMAs have completed
+  uint64_t* mma_done = done + STAGES;
   uint64_t* amax_bar = mma_done + 1;  // [4 lane quarters][2 tile parities]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 516);
@@ -134,16 +175,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], EPI_WARPS);
-    }
-    for (int s = 0; s < kScaleSlots; ++s) {
-      mbar_init(&sc_full[s], 1);
-      mbar_init(&sc_empty[s], EPI_WARPS);
+      mbar_init(&ready[s], 1 + EPI_WARPS);
+      mbar_init(&done[s], 1);
     }
     mbar_init(mma_done, 1);
     for (int b = 0; b < 8; ++b) mbar_init(&amax_bar[b], 64);
@@ -166,47 +199,39 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   const int num_tiles = p.m_tiles * p.n_tiles;
   const uint64_t deadline = globaltimer_ns() + p.timeout_ns;
 
-  // Registers (as launched 384 x 168 = 64512): the four helper warps give theirs up, the folding warps hold the
-  // 128 accumulators and two TMEM loads in flight: 128 x 48 + 256 x 224 = 63488.
+  // Registers (as launched 384 x 168 = 64512): the four helper warps give theirs up (two idle), the folding warps hold the
+  // 128 accumulators and two TMEM loads in flight: 128 x 64 + 256 x 216 = 63488.
   if (warp < EPI_BASE) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n" ::: "memory");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::: "memory");
     if (warp == 0) {
       // ---------------- TMA producer
       if (lane == 0) {
-        int stage = 0, issued = 0;
-        uint32_t phase = 0;
+        int stage = 0;
+        uint32_t phase = 0, it = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
           int m_t, n_t;
           decode_tile(p, tile, m_t, n_t);
+          const float* sa = p.sa + (int64_t)m_t * BM;
           const int b0 = SWIGLU ? n_t * 128 : n_t * BN, b1 = SWIGLU ? p.N / 2 + n_t * 128 : n_t * BN + 128;
-          for (int kb = 0; kb < KB; ++kb) {
-            if (!mbar_wait(&empty[stage], phase ^ 1u, deadline, abort_flag)) {
+          for (int kb = 0; kb < KB; ++kb, ++it) {
+            if (!mbar_wait(&done[stage], phase ^ 1u, deadline, abort_flag)) {
               ok = false;
               break;
             }
-            mbar_arrive_expect_tx(&full[stage], STAGE_TX);
-            tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, kb * BK, m_t * BM, &full[stage]);
-            tma_load_2d(sB + stage * B_BYTES, &p.tmap_b, kb * BK, b0, &full[stage]);
-            tma_load_2d(sB + stage * B_BYTES + B_HALF, &p.tmap_b, kb * BK, b1, &full[stage]);
-            ++issued;
+            const int scales = (kb == 0) + (kb + 1 < KB);
+            mbar_arrive_expect_tx(&ready[stage], STAGE_TX + scales * SCALE_BYTES);
+            tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, kb * BK, m_t * BM, &ready[stage]);
+            tma_load_2d(sB + stage * B_BYTES, &p.tmap_b, kb * BK, b0, &ready[stage]);
+            tma_load_2d(sB + stage * B_BYTES + B_HALF, &p.tmap_b, kb * BK, b1, &ready[stage]);
+            if (kb == 0) bulk_load(sSa + it % SCALE_SLOTS * BM, sa, SCALE_BYTES, &ready[stage]);
+            if (kb + 1 < KB)
+              bulk_load(sSa + (it + 1) % SCALE_SLOTS * BM, sa + (int64_t)(kb + 1) * p.mp, SCALE_BYTES, &ready[stage]);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
             }
           }
-        }
-        // the copies of the last armed stages must land before this CTA may exit
-        const uint64_t drain_deadline = globaltimer_ns() + 200000000ull;
-        volatile int no_abort = 0;
-        for (int i = 0; i < min(issued, STAGES); ++i) {
-          int s = stage - 1 - i;
-          uint32_t ph = phase;
-          if (s < 0) {
-            s += STAGES;
-            ph ^= 1u;
-          }
-          mbar_wait(&full[s], ph, drain_deadline, &no_abort);
         }
       }
     } else if (warp == 1) {
@@ -217,19 +242,17 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
           for (int kb = 0; kb < KB; ++kb, ++it) {
-            const uint32_t buf = it & 1u;
-            if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, deadline, abort_flag) ||
-                !mbar_wait(&full[stage], phase, deadline, abort_flag)) {
+            const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES), bdesc = sdesc_sw128(sB + stage * B_BYTES);
+            const uint32_t acc = tmem_base + (it & 1u) * BN;
+            if (!mbar_wait(&ready[stage], phase, deadline, abort_flag)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES), bdesc = sdesc_sw128(sB + stage * B_BYTES);
 #pragma unroll
             for (int k = 0; k < BK / 32; ++k)
-              tc_mma_f8f6f4(tmem_base + buf * BN, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, BN), k != 0);
-            tc_commit(&empty[stage]);
-            tc_commit(&acc_full[buf]);
+              tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, BN), k != 0);
+            tc_commit(&done[stage]);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -240,47 +263,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         volatile int no_abort = 0;
         mbar_wait(mma_done, 0, globaltimer_ns() + 200000000ull, &no_abort);
       }
-    } else if (warp == 2) {
-      // ---------------- scale products, four K blocks of loads in flight
-      uint32_t it = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-        int m_t, n_t;
-        decode_tile(p, tile, m_t, n_t);
-        const int nb0 = SWIGLU ? n_t : 2 * n_t, nb1 = SWIGLU ? p.NB / 2 + n_t : 2 * n_t + 1;
-        const float* sa = p.sa + (int64_t)m_t * BM + 4 * lane;
-        const float* sb0 = p.sb + (int64_t)nb0 * KB;
-        const float* sb1 = p.sb + (int64_t)nb1 * KB;
-        const bool has1 = nb1 < p.NB;
-        for (int kb = 0; ok && kb < KB; kb += 4) {
-          float4 a[4];
-          float f0[4], f1[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (kb + j < KB) {
-              a[j] = *reinterpret_cast<const float4*>(sa + (int64_t)(kb + j) * p.mp);
-              f0[j] = __ldg(sb0 + kb + j);
-              f1[j] = has1 ? __ldg(sb1 + kb + j) : 0.f;
-            }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (ok && kb + j < KB) {
-              const uint32_t slot = it % kScaleSlots;
-              ok = warp_wait(&sc_empty[slot], ((it / kScaleSlots) & 1u) ^ 1u, deadline, abort_flag);
-              if (ok) {
-                float4* dst = reinterpret_cast<float4*>(sF + slot * 2 * BM);
-                dst[lane] = make_float4(a[j].x * f0[j], a[j].y * f0[j], a[j].z * f0[j], a[j].w * f0[j]);
-                dst[32 + lane] = make_float4(a[j].x * f1[j], a[j].y * f1[j], a[j].z * f1[j], a[j].w * f1[j]);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sc_full[slot]);
-                ++it;
-              }
-            }
-        }
-      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n" ::: "memory");
     // ---------------- fold and epilogue
     const int q = warp & 3;                   // TMEM lane quarter this warp may access
     const int half = (warp - EPI_BASE) >> 2;  // which half of the tile's columns
@@ -291,54 +276,80 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
     const int col1 = SWIGLU ? 128 + 64 * half : 128 * half + 64;
     uint32_t it = 0, tcount = 0;
     bool ok = true;
+    if (lane == 0) {  // both TMEM buffers start free
+      mbar_arrive(&ready[0]);
+      mbar_arrive(&ready[1]);
+    }
     for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x, ++tcount) {
       int m_t, n_t;
       decode_tile(p, tile, m_t, n_t);
-      float acc0[64], acc1[64];
+      // the weight blocks of the two column groups (a block behind the last has no columns that are stored)
+      const int nb = SWIGLU ? n_t : min(2 * n_t + half, p.NB - 1);
+      const float* sb0 = p.sb + (int64_t)nb * KB;
+      const float* sb1 = p.sb + (int64_t)(p.NB / 2 + nb) * KB;  // SwiGLU only
+      float b0 = __ldg(sb0), b1 = SWIGLU ? __ldg(sb1) : 0.f;
+      uint64_t acc0[32], acc1[32];  // pairs of columns
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc0[i] = acc1[i] = 0.f;
+      for (int i = 0; i < 32; ++i) acc0[i] = acc1[i] = 0;
+      // 64 columns are loaded while the 64 before them are folded, across K blocks as well
+      uint32_t va[32], vb[32];
+      ok = warp_wait(&done[it % STAGES], (it / STAGES) & 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld_32x32b_x32(t_lane + (it & 1u) * BN + col0, va);
+      tmem_ld_32x32b_x32(t_lane + (it & 1u) * BN + col0 + 32, vb);
+      float sa = sSa[it % SCALE_SLOTS * BM + row_in_tile];
       for (int kb = 0; kb < KB; ++kb, ++it) {
-        const uint32_t slot = it % kScaleSlots, buf = it & 1u;
-        ok = warp_wait(&sc_full[slot], (it / kScaleSlots) & 1u, deadline, abort_flag);
-        if (!ok) break;
-        const float f0 = sF[slot * 2 * BM + (SWIGLU ? 0 : half * BM) + row_in_tile];
-        const float f1 = SWIGLU ? sF[slot * 2 * BM + BM + row_in_tile] : f0;
-        ok = warp_wait(&acc_full[buf], (it >> 1) & 1u, deadline, abort_flag);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(&sc_empty[slot]);
-        tc_fence_after();
-        const uint32_t tb = t_lane + buf * BN;
-        uint32_t va[32], vb[32];
-        tmem_ld_32x32b_x32(tb + col0, va);
-        tmem_ld_32x32b_x32(tb + col0 + 32, vb);
-        tmem_wait_ld();
+        const uint32_t tb = t_lane + (it & 1u) * BN;
+        const bool more = kb + 1 < KB;
+        const uint64_t f0 = twice(sa * b0), f1 = SWIGLU ? twice(sa * b1) : f0;
+        if (more) {  // the next block's factors; its scales landed before this block's MMAs started
+          sa = sSa[(it + 1) % SCALE_SLOTS * BM + row_in_tile];
+          b0 = __ldg(sb0 + kb + 1);
+          if (SWIGLU) b1 = __ldg(sb1 + kb + 1);
+        }
+        tmem_wait_regs(va);
+        tmem_wait_regs(vb);
         fold32(acc0, va, f0);
-        fold32(acc0 + 32, vb, f0);
         tmem_ld_32x32b_x32(tb + col1, va);
+        fold32(acc0 + 16, vb, f0);
         tmem_ld_32x32b_x32(tb + col1 + 32, vb);
-        tmem_wait_ld();
-        tc_fence_before();  // this warp's reads of the buffer are complete: hand it back to the MMA warp
+        // asked early: by the time the answer is used the next block is usually done
+        const bool early = more && mbar_try_wait(&done[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);
+        tmem_wait_regs(va);
+        tmem_wait_regs(vb);
+        tc_fence_before();  // this warp's reads of the buffer are complete: K block it + 2 may have it
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        if (lane == 0) mbar_arrive(&ready[(it + 2) % STAGES]);
+        if (more && !__all_sync(0xffffffffu, early)) {
+          ok = warp_wait(&done[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u, abort_flag);
+          if (!ok) break;
+        }
+        tc_fence_after();
+        const uint32_t tn = t_lane + ((it + 1) & 1u) * BN;
         fold32(acc1, va, f1);
-        fold32(acc1 + 32, vb, f1);
+        if (more) tmem_ld_32x32b_x32(tn + col0, va);
+        fold32(acc1 + 16, vb, f1);
+        if (more) tmem_ld_32x32b_x32(tn + col0 + 32, vb);
       }
       if (!ok) break;
       const int row0 = m_t * BM + q * 32;
       if constexpr (SWIGLU) {
         const int I = p.N / 2;
         const float lim = p.swiglu_limit;
-        float amax = 0.f;
+        float amax = 0.f, h[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          acc0[i] = swiglu(acc0[i], acc1[i], lim);
-          amax = fmaxf(amax, fabsf(acc0[i]));
+        for (int i = 0; i < 32; ++i) {
+          const float2 g = halves(acc0[i]), u = halves(acc1[i]);
+          h[2 * i] = swiglu(g.x, u.x, lim);
+          h[2 * i + 1] = swiglu(g.y, u.y, lim);
+          amax = fmaxf(amax, fmaxf(fabsf(h[2 * i]), fabsf(h[2 * i + 1])));
         }
         // the row's other 64 h values live in the partner warp (same lane quarter, other half)
         const uint32_t par = tcount & 1u;
         s_amax[(par * 2 + half) * 128 + row_in_tile] = amax;
         mbar_arrive(&amax_bar[q * 2 + par]);
-        ok = warp_wait(&amax_bar[q * 2 + par], (tcount >> 1) & 1u, deadline, abort_flag);
+        ok = warp_wait(&amax_bar[q * 2 + par], (tcount >> 1) & 1u, abort_flag);
         if (!ok) break;
         amax = fmaxf(amax, s_amax[(par * 2 + (half ^ 1)) * 128 + row_in_tile]);
         if (row0 + lane < p.M) {
@@ -346,10 +357,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           block_scale(amax, p.pow2, scale, inv);
           uint4* dst = reinterpret_cast<uint4*>(p.out_q + (int64_t)(row0 + lane) * I + n_t * 128 + half * 64);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float* h = acc0 + 16 * j;
-            dst[j] = make_uint4(codes4(h, inv), codes4(h + 4, inv), codes4(h + 8, inv), codes4(h + 12, inv));
-          }
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_uint4(codes4(h + 16 * j, inv), codes4(h + 16 * j + 4, inv), codes4(h + 16 * j + 8, inv),
+                                codes4(h + 16 * j + 12, inv));
           if (half == 0) p.out_sa[(int64_t)n_t * p.mp + row0 + lane] = scale;
         }
       } else {
@@ -359,10 +369,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         const bool fp16 = p.out_fp16 != 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float* a = c < 2 ? acc0 + 32 * c : acc1 + 32 * (c - 2);
+          const uint64_t* a = c < 2 ? acc0 + 16 * c : acc1 + 16 * (c - 2);
           uint32_t o[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = pack16(a[2 * i], a[2 * i + 1], fp16);
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = halves(a[i]);
+            o[i] = pack16(v.x, v.y, fp16);
+          }
           store_rows(o, wb, out0 + 32 * c, p.ldo, p.M - row0, p.N - c0 - 32 * c, lane);
         }
       }
@@ -370,7 +383,12 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) report(p.status, status_word(ASAP_ST_PIPELINE_TIMEOUT, 0, 0, 16 + SWIGLU));
+  if (*abort_flag) {  // copies may still be on their way into this block's shared memory: let them land before it ends
+    if (threadIdx.x == 0) report(p.status, status_word(ASAP_ST_PIPELINE_TIMEOUT, 0, 0, 16 + SWIGLU));
+    const uint64_t landed = globaltimer_ns() + 200000000ull;
+    while (globaltimer_ns() < landed) {
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);

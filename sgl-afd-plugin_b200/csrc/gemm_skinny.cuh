@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(SK_THREADS, Skinny<TN, SWIGLU>::C <= 32 ? 2 : 
     for (int i = 0; i < C; ++i) acc[i] = 0.f;
     for (int i = 0; i < kbs; ++i) {
       const uint32_t buf = i % T::BUFS;
-      ok = warp_wait(&x_full[i], 0, deadline, abort_flag) &&
-           warp_wait(&acc_full[buf], (i / T::BUFS) & 1u, deadline, abort_flag);
+      ok = warp_wait(&x_full[i], 0, abort_flag) &&
+           warp_wait(&acc_full[buf], (i / T::BUFS) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const float sb = sSb[2 * i + (SWIGLU ? part : 0)];
