@@ -347,15 +347,15 @@ int asap_ffn_debug_ptrs(uint64_t ws_handle, uint64_t* expert_counts, uint64_t* p
 /* ------------------------------------------------------------------ the attention rank's half of the layer
  * FP8 block-scaled linear: W [n, k] E4M3 bytes (checkpoint order) with one fp32 scale per 128 x 128 block, [ceil(n /
  * 128), ceil(k / 128)]; n and k multiples of 16 (the last blocks may be partial).  Activations are quantised per row
- * and 128 values of K: scale = amax / 448, codes = e4m3(x * (448 / amax)); with pow2 the scale is rounded up to a power
- * of two and codes = e4m3(x / scale) (for weights whose scales are E8M0, given here as the fp32 values they stand
- * for). */
+ * and 128 values of K: scale = amax / 448, codes = e4m3(x * (448 / amax)).  Weights whose scales are E8M0 give them
+ * twice: `scale` as the fp32 values they stand for, and `atoms`, the layout the block-scaled MMA reads, [ceil(k / 128),
+ * ceil(n / 128) rounded up to even, 512] with each scale's byte 512 times; the activations' scales are then rounded up to
+ * powers of two and codes = e4m3(x / scale).  atoms = 0: fp32 scales. */
 #define ASAP_LINEAR_MAX_ROWS (1 << 20)
 #define ASAP_LINEAR_MAX_DIM (1 << 17)
 typedef struct {
   int32_t n, k;
-  uint64_t w, scale;
-  int32_t pow2, pad;
+  uint64_t w, scale, atoms;
 } asap_fp8_linear_t;
 int asap_fp8_linear_register(const asap_fp8_linear_t* d, uint64_t* handle);
 int asap_fp8_linear_release(uint64_t handle);

@@ -54,8 +54,7 @@ class Fp8Experts_t(ctypes.Structure):
 
 
 class Fp8Linear_t(ctypes.Structure):
-    _fields_ = [("n", c_int32), ("k", c_int32), ("w", c_uint64), ("scale", c_uint64), ("pow2", c_int32),
-                ("pad", c_int32)]
+    _fields_ = [("n", c_int32), ("k", c_int32), ("w", c_uint64), ("scale", c_uint64), ("atoms", c_uint64)]
 
 
 class Route_t(ctypes.Structure):

@@ -50,6 +50,15 @@ def check(device: int = 0) -> None:
             raise N.AsapError("asap_fp8_linear", N.ASAP_ETIMEOUT, f"device status {N.decode_status(value)}")
 
 
+def _scale_atoms(scale: torch.Tensor) -> torch.Tensor:
+    """E8M0 scales [nb, kb] -> uint8 [kb, nb rounded up to even, 512], each byte 512 times (1/32 of the weight)."""
+    b = scale.view(torch.uint8)
+    nb, kb = b.shape
+    atoms = torch.zeros((kb, nb + nb % 2, 512), dtype=torch.uint8, device=b.device)
+    atoms[:, :nb] = b.t()[:, :, None]
+    return atoms
+
+
 class _Weight:
     """A registered [n, k] weight (keeps its tensors alive)."""
 
@@ -73,8 +82,10 @@ class _Weight:
         self.pow2 = scale.dtype == torch.float8_e8m0fnu
         self.w, self.scale = w, scale.float().contiguous()
         self.device = w.device
+        self.atoms = _scale_atoms(scale) if self.pow2 else None
         self.handle = 0
-        desc = N.Fp8Linear_t(self.n, self.k, self.w.data_ptr(), self.scale.data_ptr(), int(self.pow2), 0)
+        desc = N.Fp8Linear_t(self.n, self.k, self.w.data_ptr(), self.scale.data_ptr(),
+                             self.atoms.data_ptr() if self.pow2 else 0)
         h = ctypes.c_uint64()
         with torch.cuda.device(self.device):
             N.call("asap_fp8_linear_register", ctypes.byref(desc), ctypes.byref(h))

@@ -43,6 +43,9 @@ struct Params {
   CUtensorMap tmap_b;  // weights [N, K]
   const float* sa;     // activation scales [K blocks][mp]
   const float* sb;     // weight scales [N blocks][K blocks]
+  const uint8_t* sfa;  // the same two as E8M0 atoms (linear_pow2_kernel): [mp / 128][K blocks] and
+  const uint8_t* sfb;  // [K blocks][nb_atoms]
+  int32_t nb_atoms;
   int64_t mp;          // M rounded up to 128
   int32_t M, N, KB, NB, m_tiles, n_tiles;
   void* out;           // linear: [M, N], bf16 or fp16
@@ -51,7 +54,6 @@ struct Params {
   float swiglu_limit;  // SwiGLU: N = 2I, gate rows then up rows
   uint8_t* out_q;      // SwiGLU: codes of h [M, I]
   float* out_sa;       // SwiGLU: scales of h [I / 128][mp]
-  int32_t pow2;        // scales of h are powers of two
   uint64_t status, timeout_ns;
 };
 
@@ -82,6 +84,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     }
   }
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// The same lane of a converged warp each time (the lane whose commits track its MMAs), as a predicate ptxas knows to be
+// one thread's.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // tcgen05.wait::ld that the uses of `r` cannot be moved above
@@ -172,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 516);
   float* s_amax = reinterpret_cast<float*>(ctrl + 1024);  // [2 tile parities][2 halves][128 rows]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ready[s], 1 + EPI_WARPS);
@@ -235,8 +245,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         }
       }
     } else if (warp == 1) {
-      // ---------------- MMA issuer: one K block per TMEM buffer, alternating
-      if (lane == 0) {
+      // ---------------- MMA issuer: one K block per TMEM buffer, alternating.  The warp runs the loop as a whole and one
+      // elected lane issues, so that descriptors stay in uniform registers (1057 -> 1009 cycles per K block).
+      {
         int stage = 0;
         uint32_t phase = 0, it = 0;
         bool ok = true;
@@ -244,22 +255,24 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           for (int kb = 0; kb < KB; ++kb, ++it) {
             const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES), bdesc = sdesc_sw128(sB + stage * B_BYTES);
             const uint32_t acc = tmem_base + (it & 1u) * BN;
-            if (!mbar_wait(&ready[stage], phase, deadline, abort_flag)) {
-              ok = false;
-              break;
-            }
+            ok = __all_sync(0xffffffffu, mbar_wait(&ready[stage], phase, deadline, abort_flag));
+            if (!ok) break;
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / 32; ++k)
-              tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, BN), k != 0);
-            tc_commit(&done[stage]);
+              for (int k = 0; k < BK / 32; ++k)
+                tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, BN), k != 0);
+              tc_commit(&done[stage]);
+            }
+            __syncwarp();
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
             }
           }
         }
-        tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
+        if (elect_one()) tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
+        __syncwarp();
         volatile int no_abort = 0;
         mbar_wait(mma_done, 0, globaltimer_ns() + 200000000ull, &no_abort);
       }
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         amax = fmaxf(amax, s_amax[(par * 2 + (half ^ 1)) * 128 + row_in_tile]);
         if (row0 + lane < p.M) {
           float scale, inv;
-          block_scale(amax, p.pow2, scale, inv);
+          block_scale(amax, false, scale, inv);
           uint4* dst = reinterpret_cast<uint4*>(p.out_q + (int64_t)(row0 + lane) * I + n_t * 128 + half * 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j)

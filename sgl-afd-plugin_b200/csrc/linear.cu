@@ -72,13 +72,15 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 }  // namespace lin
 
 #include "gemm_linear.cuh"
+#include "gemm_pow2.cuh"
 #include "gemm_skinny.cuh"
 
 namespace lin {
 
 // ------------------------------------------------------------------ activation quantisation
-// x [M, K] -> codes [M, 128 * KB] (K padded with 0) and scales [KB][mp].  A warp takes 256 values of one row per
-// step, 8 per lane; a half-warp holds a block.
+// x [M, K] -> codes [M, 128 * KB] (K padded with 0) and scales: fp32 [KB][mp], or E8M0 atoms when they are powers of
+// two.  A half-warp holds a block, 8 values per lane.  Bound by memory; a warp has QUANT_AHEAD loads of 512 bytes in
+// flight before it uses the first.
 struct QuantArgs {
   const uint16_t* x;
   int64_t ldx;
@@ -88,21 +90,38 @@ struct QuantArgs {
   float* sa;
 };
 
+constexpr int QUANT_AHEAD = 4;
 __global__ void __launch_bounds__(256) quant_rows_kernel(const __grid_constant__ QuantArgs p) {
   const int lane = threadIdx.x & 31;
-  const int chunks = (p.KB + 1) / 2;
+  const int chunks = (p.KB + 1) / 2;  // of 256 values
   const int64_t items = (int64_t)p.M * chunks, step = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < items; i += step) {
-    const int64_t row = i / chunks;
-    const int col = (int)(i - row * chunks) * 256 + lane * 8;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (col < p.K) u = *reinterpret_cast<const uint4*>(p.x + row * p.ldx + col);
-    uint2 codes;
-    float scale;
-    quant8(u, p.fp16 != 0, p.pow2 != 0, codes, scale);
-    if (col < p.KB * 128) {
-      *reinterpret_cast<uint2*>(p.xq + row * p.KB * 128 + col) = codes;
-      if ((lane & 15) == 0) p.sa[(int64_t)(col / 128) * p.mp + row] = scale;
+  for (int64_t i0 = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i0 < items; i0 += QUANT_AHEAD * step) {
+    uint4 u[QUANT_AHEAD];
+    int64_t row[QUANT_AHEAD];
+    int col[QUANT_AHEAD];
+#pragma unroll
+    for (int j = 0; j < QUANT_AHEAD; ++j) {
+      const int64_t i = i0 + j * step;
+      row[j] = i / chunks;
+      col[j] = (int)(i - row[j] * chunks) * 256 + lane * 8;
+      u[j] = make_uint4(0, 0, 0, 0);
+      if (i < items && col[j] < p.K) u[j] = *reinterpret_cast<const uint4*>(p.x + row[j] * p.ldx + col[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < QUANT_AHEAD; ++j) {
+      uint2 codes;
+      float scale;
+      quant8(u[j], p.fp16 != 0, p.pow2 != 0, codes, scale);
+      if (i0 + j * step < items && col[j] < p.KB * 128) {
+        *reinterpret_cast<uint2*>(p.xq + row[j] * p.KB * 128 + col[j]) = codes;
+        if ((lane & 15) == 0) {
+          const int kb = col[j] / 128;
+          if (p.pow2)
+            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.sa) + atom_off(row[j], kb, p.KB)) =
+                atom_word(scale);
+          else p.sa[(int64_t)kb * p.mp + row[j]] = scale;
+        }
+      }
     }
   }
 }
@@ -133,6 +152,8 @@ static int ensure_attrs() {
   if (dev >= 0 && dev < 64 && done[dev]) return ASAP_OK;
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
+  ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
   for (const void* f : {(const void*)linear_skinny_kernel<16, 0>, (const void*)linear_skinny_kernel<32, 0>,
                         (const void*)linear_skinny_kernel<64, 0>, (const void*)linear_skinny_kernel<128, 0>,
                         (const void*)linear_skinny_kernel<16, 1>, (const void*)linear_skinny_kernel<32, 1>,
@@ -184,7 +205,7 @@ static int quantise(uint64_t x, int64_t ldx, int32_t m, const Linear* L, int32_t
   q.K = L->d.k;
   q.KB = L->KB;
   q.fp16 = fp16;
-  q.pow2 = L->d.pow2;
+  q.pow2 = L->d.atoms != 0;
   q.mp = mp;
   q.xq = (uint8_t*)xq;
   q.sa = (float*)sa;
@@ -207,6 +228,9 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
   p.tmap_b = L->map;
   p.sa = (const float*)sa;
   p.sb = (const float*)L->d.scale;
+  p.sfa = (const uint8_t*)sa;
+  p.sfb = (const uint8_t*)L->d.atoms;
+  p.nb_atoms = (L->NB + 1) / 2 * 2;
   p.mp = mp;
   p.M = m;
   p.N = L->d.n;
@@ -220,11 +244,16 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
   p.swiglu_limit = limit;
   p.out_q = (uint8_t*)out_q;
   p.out_sa = (float*)out_sa;
-  p.pow2 = L->d.pow2;
   p.status = status;
   p.timeout_ns = timeout_ns;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
+  if (L->d.atoms) {
+    if (swiglu) linear_pow2_kernel<1><<<grid, P2_THREADS, P2_SMEM_BYTES, st>>>(p);
+    else linear_pow2_kernel<0><<<grid, P2_THREADS, P2_SMEM_BYTES, st>>>(p);
+    ASAP_CHECK_LAUNCH("linear_pow2_kernel");
+    return ASAP_OK;
+  }
   if (swiglu) linear_gemm_kernel<1><<<grid, THREADS, SMEM_BYTES, st>>>(p);
   else linear_gemm_kernel<0><<<grid, THREADS, SMEM_BYTES, st>>>(p);
   ASAP_CHECK_LAUNCH("linear_gemm_kernel");
@@ -283,7 +312,7 @@ static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, cudaSt
   p.stages = pl.stages;
   p.max_kb = pl.max_kb;
   p.sb = (const float*)L->d.scale;
-  p.pow2 = L->d.pow2;
+  p.pow2 = L->d.atoms != 0;
   const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(n_tiles * pl.split, (p.M + pl.tn - 1) / pl.tn);
@@ -322,8 +351,8 @@ int asap_fp8_linear_register(const asap_fp8_linear_t* d, uint64_t* handle) {
               ASAP_LINEAR_MAX_DIM, d->n, d->k);
     return ASAP_EINVAL;
   }
-  if (!d->w || (d->w & 15) || !d->scale || (d->scale & 3)) {
-    set_error("asap_fp8_linear_register: weights must be 16-byte and scales 4-byte aligned, non-NULL");
+  if (!d->w || (d->w & 15) || !d->scale || (d->scale & 3) || (d->atoms & 15)) {
+    set_error("asap_fp8_linear_register: weights must be 16-byte and scales 4-byte aligned, non-NULL, atoms 16-byte");
     return ASAP_EINVAL;
   }
   lin::Linear* L = new (std::nothrow) lin::Linear;
@@ -413,7 +442,7 @@ int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t
               (unsigned long long)w2_handle);
     return ASAP_EINVAL;
   }
-  if (L13->d.n % 256 || L2->d.k != L13->d.n / 2 || L2->d.n != L13->d.k || L13->d.pow2 != L2->d.pow2) {
+  if (L13->d.n % 256 || L2->d.k != L13->d.n / 2 || L2->d.n != L13->d.k || !L13->d.atoms != !L2->d.atoms) {
     set_error("asap_fp8_shared: w13 [%d, %d] and w2 [%d, %d] are not [2I, H] and [H, I] with I %% 128 == 0 and scales "
               "of one kind", L13->d.n, L13->d.k, L2->d.n, L2->d.k);
     return ASAP_EINVAL;
