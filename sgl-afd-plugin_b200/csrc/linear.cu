@@ -84,7 +84,7 @@ namespace lin {
 struct QuantArgs {
   const uint16_t* x;
   int64_t ldx;
-  int32_t M, K, KB, fp16, pow2;
+  int32_t M, K, KB, fp16, pow2, atoms;
   int64_t mp;
   uint8_t* xq;
   float* sa;
@@ -93,33 +93,34 @@ struct QuantArgs {
 constexpr int QUANT_AHEAD = 4;
 __global__ void __launch_bounds__(256) quant_rows_kernel(const __grid_constant__ QuantArgs p) {
   const int lane = threadIdx.x & 31;
-  const int chunks = (p.KB + 1) / 2;  // of 256 values
-  const int64_t items = (int64_t)p.M * chunks, step = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t i0 = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i0 < items; i0 += QUANT_AHEAD * step) {
+  const uint32_t groups = (p.KB + 2 * QUANT_AHEAD - 1) / (2 * QUANT_AHEAD);  // of QUANT_AHEAD x 256 values
+  const uint32_t items = p.M * groups, step = gridDim.x * (blockDim.x >> 5);
+  grid_dependents_launch();
+  for (uint32_t i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < items; i += step) {
+    const uint32_t row = i / groups;
+    const int col0 = (int)(i - row * groups) * QUANT_AHEAD * 256 + lane * 8;
+    const uint16_t* x = p.x + (int64_t)row * p.ldx;
     uint4 u[QUANT_AHEAD];
-    int64_t row[QUANT_AHEAD];
-    int col[QUANT_AHEAD];
 #pragma unroll
     for (int j = 0; j < QUANT_AHEAD; ++j) {
-      const int64_t i = i0 + j * step;
-      row[j] = i / chunks;
-      col[j] = (int)(i - row[j] * chunks) * 256 + lane * 8;
+      const int col = col0 + 256 * j;
       u[j] = make_uint4(0, 0, 0, 0);
-      if (i < items && col[j] < p.K) u[j] = *reinterpret_cast<const uint4*>(p.x + row[j] * p.ldx + col[j]);
+      if (col < p.K) u[j] = *reinterpret_cast<const uint4*>(x + col);
     }
 #pragma unroll
     for (int j = 0; j < QUANT_AHEAD; ++j) {
+      const int col = col0 + 256 * j;
+      if (col - lane * 8 >= p.KB * 128) break;
       uint2 codes;
       float scale;
       quant8(u[j], p.fp16 != 0, p.pow2 != 0, codes, scale);
-      if (i0 + j * step < items && col[j] < p.KB * 128) {
-        *reinterpret_cast<uint2*>(p.xq + row[j] * p.KB * 128 + col[j]) = codes;
+      if (col < p.KB * 128) {
+        *reinterpret_cast<uint2*>(p.xq + (int64_t)row * p.KB * 128 + col) = codes;
         if ((lane & 15) == 0) {
-          const int kb = col[j] / 128;
-          if (p.pow2)
-            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.sa) + atom_off(row[j], kb, p.KB)) =
-                atom_word(scale);
-          else p.sa[(int64_t)kb * p.mp + row[j]] = scale;
+          const int kb = col / 128;
+          if (p.atoms)
+            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.sa) + atom_off(row, kb, p.KB)) = atom_word(scale);
+          else p.sa[(int64_t)kb * p.mp + row] = scale;
         }
       }
     }
@@ -154,11 +155,13 @@ static int ensure_attrs() {
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
-  for (const void* f : {(const void*)linear_skinny_kernel<16, 0>, (const void*)linear_skinny_kernel<32, 0>,
-                        (const void*)linear_skinny_kernel<64, 0>, (const void*)linear_skinny_kernel<128, 0>,
-                        (const void*)linear_skinny_kernel<16, 1>, (const void*)linear_skinny_kernel<32, 1>,
-                        (const void*)linear_skinny_kernel<64, 1>})
+  for (const void* f : {(const void*)linear_skinny_kernel<16, 0, 0>, (const void*)linear_skinny_kernel<16, 0, 1>,
+                        (const void*)linear_skinny_kernel<32, 0, 1>, (const void*)linear_skinny_kernel<64, 0, 1>,
+                        (const void*)linear_skinny_kernel<128, 0, 1>, (const void*)linear_skinny_kernel<16, 1, 1>,
+                        (const void*)linear_skinny_kernel<32, 1, 1>, (const void*)linear_skinny_kernel<64, 1, 1>}) {
     ASAP_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    ASAP_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  }
   if (dev >= 0 && dev < 64) done[dev] = true;
   return ASAP_OK;
 }
@@ -196,8 +199,8 @@ static int check_rows(const char* fn, int32_t m, uint64_t x, int64_t ldx, int32_
   return ASAP_OK;
 }
 
-static int quantise(uint64_t x, int64_t ldx, int32_t m, const Linear* L, int32_t fp16, uint64_t xq, uint64_t sa,
-                    int64_t mp, cudaStream_t st) {
+static int quantise(uint64_t x, int64_t ldx, int32_t m, const Linear* L, int32_t fp16, bool atoms, uint64_t xq,
+                    uint64_t sa, int64_t mp, cudaStream_t st) {
   QuantArgs q{};
   q.x = (const uint16_t*)x;
   q.ldx = ldx;
@@ -206,10 +209,11 @@ static int quantise(uint64_t x, int64_t ldx, int32_t m, const Linear* L, int32_t
   q.KB = L->KB;
   q.fp16 = fp16;
   q.pow2 = L->d.atoms != 0;
+  q.atoms = atoms;
   q.mp = mp;
   q.xq = (uint8_t*)xq;
   q.sa = (float*)sa;
-  const int64_t items = (int64_t)m * ((L->KB + 1) / 2);
+  const int64_t items = (int64_t)m * ((L->KB + 2 * QUANT_AHEAD - 1) / (2 * QUANT_AHEAD));
   const int64_t blocks = (items + 7) / 8, cap = 8ll * sm_count();
   quant_rows_kernel<<<(int)(blocks < cap ? blocks : cap), 256, 0, st>>>(q);
   ASAP_CHECK_LAUNCH("quant_rows_kernel");
@@ -261,49 +265,122 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
 }
 
 // ------------------------------------------------------------------ few rows
-// How a product of few rows is launched, or split = 0: not at all.
+// Up to here the few-rows linear quantises its rows itself.  7168 x 4096: 1 row 10.8 us against 11.0 with a kernel before
+// it (2064 x 1040: 5.3 against 5.8), and one launch less for the caller; 8 rows 13.1 against 11.7.
+constexpr int kInKernelRows = 4;
+
+// How a product of few rows is launched.  rounds: K blocks that a CTA works through, times the waves of clusters.
 struct SkinnyPlan {
-  int tn, split, stages, max_kb, smem;
+  int tmpl, tn, split, stages, max_kb, smem;
+  int64_t rounds;
+  explicit operator bool() const { return split > 0; }
 };
 
-// TN is the smallest of 16, 32, 64, 128 that holds the rows (64 at most with SwiGLU, whose tiles are two), halved while
-// a CTA's part of x does not fit beside the fewest stages.  K is split as far as the grid stays within two CTAs per SM.
-template <int SWIGLU>
-static SkinnyPlan skinny_plan(const Linear* L, int32_t m) {
-  const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
-  int tn = m <= 16 ? 16 : m <= 32 ? 32 : (m <= 64 || SWIGLU) ? 64 : 128;
-  for (; tn >= 16; tn /= 2) {
-    const int64_t y = (m + tn - 1) / tn;
-    int split = 1;
-    while (split < SK_MAX_SPLIT && 2 * split <= L->KB && n_tiles * y * split * 2 <= 2 * sm_count()) split *= 2;
-    for (; split <= SK_MAX_SPLIT && split <= L->KB; split *= 2) {
-      SkinnyPlan pl;
-      pl.tn = tn;
-      pl.split = split;
-      pl.max_kb = (L->KB + split - 1) / split;
-      const int tiles = SWIGLU ? 2 : 1, stage = tiles * 128 * BK, part = tiles * tn * 512;
-      const int least = part > 3 * stage ? (part + stage - 1) / stage : 3;
-      const int fixed = 1024 + 2048 + pl.max_kb * (tn * BK + tn * 4 + 8);
-      if (pl.max_kb > SK_MAX_KB || fixed + least * stage > kMaxSmem) continue;
-      // half an SM's shared memory if three stages fit it, so that two CTAs share the SM
-      const int half = kMaxSmem / 2 - 1024;
-      const int room = tiles * tn <= 64 && fixed + least * stage <= half ? half : kMaxSmem;
-      pl.stages = (room - fixed) / stage;
-      if (pl.stages > SK_MAX_STAGES) pl.stages = SK_MAX_STAGES;
-      if (pl.stages > pl.max_kb) pl.stages = pl.max_kb;
-      if (pl.stages < least) pl.stages = least;
-      pl.smem = fixed + pl.stages * stage;
-      // never three CTAs on an SM: the third would wait for tensor memory while its cluster waits for it
-      if (pl.smem < 80 * 1024) pl.smem = 80 * 1024;
-      return pl;
+// Clusters of `split` CTAs that run at once, with two CTAs (half an SM's shared memory) or one on an SM.  A cluster lies
+// within one GPC, so eight to a cluster leave SMs idle that two would use.
+static int clusters_at_once(int split, bool two) {
+  static std::mutex mu;
+  static int cached[64][4] = {};
+  int dev = 0, log = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = cached[dev][log];
+  if (!n) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(split * 1024);
+    cfg.blockDim = dim3(SK_THREADS);
+    cfg.dynamicSmemBytes = kMaxSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, linear_skinny_kernel<16, 0, 0>, &cfg) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = sm_count() / split;
     }
   }
-  return SkinnyPlan{0, 0, 0, 0, 0};
+  return two ? 2 * n : n;  // the query knows nothing of two: it answers one CTA to an SM for whatever uses tensor memory
 }
 
-template <int SWIGLU>
-static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, cudaStream_t st) {
+// The rows are cut into equal column tiles of the MMA, of at most 128 (64 with SwiGLU, whose weight tiles are two), and
+// the kernel is compiled for 16, 32, 64 and 128.  K is split as far as all clusters still run at once: with two CTAs on an
+// SM where a folding warp holds at most 32 columns and three stages fit half an SM's shared memory, else one.
+template <int SWIGLU, int XTMA>
+static SkinnyPlan skinny_plan(const Linear* L, int32_t m) {
+  const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
+  for (int cap = XTMA ? (SWIGLU ? 64 : 128) : 16; cap >= 16; cap /= 2) {
+    const int64_t y = (m + cap - 1) / cap;
+    if (y > 65535) continue;
+    SkinnyPlan pl{};
+    pl.tn = ((int)((m + y - 1) / y) + 15) / 16 * 16;
+    pl.tmpl = pl.tn <= 16 ? 16 : pl.tn <= 32 ? 32 : pl.tn <= 64 ? 64 : 128;
+    const int tiles = SWIGLU ? 2 : 1;
+    const int stage = tiles * 128 * BK + (XTMA ? pl.tmpl * BK : 0), part = tiles * pl.tmpl * 512;
+    const int least = part > 3 * stage ? (part + stage - 1) / stage : 3;
+    const int half = kMaxSmem / 2 - 1024;
+    auto fixed = [&](int split) {
+      return 1024 + 2048 + (L->KB + split - 1) / split * ((XTMA ? 0 : pl.tmpl * BK) + pl.tmpl * 4 + 8);
+    };
+    auto two = [&](int split) { return tiles * pl.tmpl <= 64 && fixed(split) + least * stage <= half; };
+    auto fits = [&](int split) {
+      return (L->KB + split - 1) / split <= SK_MAX_KB && fixed(split) + least * stage <= kMaxSmem;
+    };
+    pl.split = 1;
+    while (2 * pl.split <= SK_MAX_SPLIT && 2 * pl.split <= L->KB &&
+           (!fits(pl.split) || n_tiles * y <= clusters_at_once(2 * pl.split, two(2 * pl.split))))
+      pl.split *= 2;
+    if (!fits(pl.split)) continue;
+    const int at_once = clusters_at_once(pl.split, two(pl.split));
+    pl.max_kb = (L->KB + pl.split - 1) / pl.split;
+    pl.rounds = (n_tiles * y + at_once - 1) / at_once * pl.max_kb;
+    pl.stages = ((two(pl.split) ? half : kMaxSmem) - fixed(pl.split)) / stage;
+    if (pl.stages > SK_MAX_STAGES) pl.stages = SK_MAX_STAGES;
+    if (pl.stages > pl.max_kb) pl.stages = pl.max_kb;
+    if (pl.stages < least) pl.stages = least;
+    pl.smem = fixed(pl.split) + pl.stages * stage;
+    // Never more CTAs on an SM than its tensor memory holds, of one launch or of two on different streams: a CTA that
+    // waits for tensor memory holds up its cluster, which may hold what another one waits for.  Two with 256 columns
+    // (80 KB: a third does not fit the SM's 228 KB), one with 512 (150 KB: not beside one of 80 either).
+    const int alone = (tiles * pl.tmpl <= 64 ? 80 : 150) * 1024;
+    if (pl.smem < alone) pl.smem = alone;
+    return pl;
+  }
+  return SkinnyPlan{};
+}
+
+// The same measure of the product in 128 x 256 tiles.  A K block takes either kernel 0.6 to 0.7 us, so the one with fewer
+// rounds is taken: 7168 x 4096 with 256 rows 26.9 us against 39.4 (28 rounds, 56), with 384 rows 45.2 against 40.1 (56, 56).
+static int64_t tile_rounds(const Linear* L, bool swiglu, int32_t m) {
+  const int64_t tiles = (int64_t)((m + BM - 1) / BM) * (swiglu ? L->d.n / 256 : (L->d.n + BN - 1) / BN);
+  return (tiles + sm_count() - 1) / sm_count() * L->KB;
+}
+
+// What is the same for every launch of a call
+static SkinnyParams skinny_params(uint64_t x, int64_t ldx, int32_t m, int32_t fp16, int64_t mp, uint64_t status,
+                                  uint64_t timeout_ns) {
+  SkinnyParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = (const uint16_t*)x;
+  p.ldx = ldx;
+  p.M = m;
+  p.fp16 = fp16;
+  p.mp = mp;
+  p.status = status;
+  p.timeout_ns = timeout_ns;
+  return p;
+}
+
+// xq / sa: the quantised rows (XTMA), from a kernel launched just before on the same stream
+template <int SWIGLU, int XTMA>
+static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, uint64_t xq, uint64_t sa, cudaStream_t st) {
   p.tmap_w = L->map;
+  if (XTMA)
+    if (int rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (const void*)xq, (uint64_t)L->KB * 128, p.M,
+                              (uint64_t)L->KB * 128, BK, pl.tn, "activation codes"))
+      return rc;
+  p.sa = (const float*)sa;
   p.K = L->d.k;
   p.N = L->d.n;
   p.KB = L->KB;
@@ -311,6 +388,7 @@ static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, cudaSt
   p.split = pl.split;
   p.stages = pl.stages;
   p.max_kb = pl.max_kb;
+  p.tn = pl.tn;
   p.sb = (const float*)L->d.scale;
   p.pow2 = L->d.atoms != 0;
   const int n_tiles = SWIGLU ? L->d.n / 256 : (L->d.n + 127) / 128;
@@ -319,20 +397,22 @@ static int skinny(const Linear* L, const SkinnyPlan& pl, SkinnyParams& p, cudaSt
   cfg.blockDim = dim3(SK_THREADS);
   cfg.dynamicSmemBytes = pl.smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = pl.split;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (pl.tn == 16) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<16, SWIGLU>, p));
-  else if (pl.tn == 32) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<32, SWIGLU>, p));
-  else if (pl.tn == 64) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<64, SWIGLU>, p));
-  else if constexpr (!SWIGLU) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<128, 0>, p));
+  cfg.numAttrs = XTMA ? 2 : 1;
+  if (pl.tmpl == 16) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<16, SWIGLU, XTMA>, p));
+  else if constexpr (XTMA) {
+    if (pl.tmpl == 32) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<32, SWIGLU, 1>, p));
+    else if (pl.tmpl == 64) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<64, SWIGLU, 1>, p));
+    else if constexpr (!SWIGLU) ASAP_CUDA(cudaLaunchKernelEx(&cfg, linear_skinny_kernel<128, 0, 1>, p));
+  }
   return ASAP_OK;
 }
-
-constexpr int kSkinnyRows = 64;  // at most this many rows take the few-rows kernel
 
 }  // namespace lin
 }  // namespace asap
@@ -409,22 +489,19 @@ int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t
   if (int rc = lin::check_rows("asap_fp8_linear", m, x, ldx, L->d.k, out, ws, ws_bytes, need)) return rc;
   if (int rc = lin::ensure_attrs()) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (m <= lin::kSkinnyRows) {
-    const lin::SkinnyPlan pl = lin::skinny_plan<0>(L, m);
-    if (pl.split) {
-      lin::SkinnyParams p{};
-      p.x = (const uint16_t*)x;
-      p.ldx = ldx;
-      p.M = m;
-      p.fp16 = fp16;
-      p.out = (void*)out;
-      p.status = status;
-      p.timeout_ns = timeout_ns;
-      return lin::skinny<0>(L, pl, p, st);
-    }
-  }
   const lin::ActWs a = lin::act_ws(m, L->d.k);
-  if (int rc = lin::quantise(x, ldx, m, L, fp16, ws, ws + a.codes, a.mp, st)) return rc;
+  lin::SkinnyParams p = lin::skinny_params(x, ldx, m, fp16, a.mp, status, timeout_ns);
+  p.out = (void*)out;
+  if (m <= lin::kInKernelRows) {
+    const lin::SkinnyPlan pl = lin::skinny_plan<0, 0>(L, m);
+    if (pl) return lin::skinny<0, 0>(L, pl, p, 0, 0, st);
+  }
+  const lin::SkinnyPlan pl = lin::skinny_plan<0, 1>(L, m);
+  if (pl && pl.rounds < lin::tile_rounds(L, false, m)) {
+    if (int rc = lin::quantise(x, ldx, m, L, fp16, false, ws, ws + a.codes, a.mp, st)) return rc;
+    return lin::skinny<0, 1>(L, pl, p, ws, ws + a.codes, st);
+  }
+  if (int rc = lin::quantise(x, ldx, m, L, fp16, L->d.atoms != 0, ws, ws + a.codes, a.mp, st)) return rc;
   return lin::product(L, false, ws, ws + a.codes, m, a.mp, out, L->d.n, fp16, 0.f, 0, 0, status, timeout_ns, st);
 }
 
@@ -454,29 +531,18 @@ int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t
   cudaStream_t st = (cudaStream_t)stream;
   const lin::ActWs a = lin::act_ws(m, H), b = lin::act_ws(m, I);
   const uint64_t sa = ws + a.codes, hq = sa + a.scales, sh = hq + b.codes;
-  if (m <= lin::kSkinnyRows) {
-    const lin::SkinnyPlan up = lin::skinny_plan<1>(L13, m), down = lin::skinny_plan<0>(L2, m);
-    if (up.split && down.split) {
-      lin::SkinnyParams p{};
-      p.x = (const uint16_t*)x;
-      p.ldx = ldx;
-      p.M = m;
-      p.fp16 = fp16;
-      p.swiglu_limit = swiglu_limit;
-      p.out_q = (uint8_t*)hq;
-      p.out_sa = (float*)sh;
-      p.mp = b.mp;
-      p.status = status;
-      p.timeout_ns = timeout_ns;
-      if (int rc = lin::skinny<1>(L13, up, p, st)) return rc;
-      p.x = nullptr;
-      p.xq = (const uint8_t*)hq;
-      p.sa = (const float*)sh;
-      p.out = (void*)out;
-      return lin::skinny<0>(L2, down, p, st);
-    }
+  const lin::SkinnyPlan up = lin::skinny_plan<1, 1>(L13, m), down = lin::skinny_plan<0, 1>(L2, m);
+  if (up && down && up.rounds + down.rounds < lin::tile_rounds(L13, true, m) + lin::tile_rounds(L2, false, m)) {
+    lin::SkinnyParams p = lin::skinny_params(x, ldx, m, fp16, a.mp, status, timeout_ns);
+    p.swiglu_limit = swiglu_limit;
+    p.out_q = (uint8_t*)hq;
+    p.out_sa = (float*)sh;
+    p.out = (void*)out;
+    if (int rc = lin::quantise(x, ldx, m, L13, fp16, false, ws, sa, a.mp, st)) return rc;
+    if (int rc = lin::skinny<1, 1>(L13, up, p, ws, sa, st)) return rc;
+    return lin::skinny<0, 1>(L2, down, p, hq, sh, st);
   }
-  if (int rc = lin::quantise(x, ldx, m, L13, fp16, ws, sa, a.mp, st)) return rc;
+  if (int rc = lin::quantise(x, ldx, m, L13, fp16, L13->d.atoms != 0, ws, sa, a.mp, st)) return rc;
   if (int rc = lin::product(L13, true, ws, sa, m, a.mp, 0, 0, fp16, swiglu_limit, hq, sh, status, timeout_ns, st))
     return rc;
   return lin::product(L2, false, hq, sh, m, b.mp, out, H, fp16, 0.f, 0, 0, status, timeout_ns, st);
