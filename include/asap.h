@@ -361,8 +361,8 @@ int asap_fp8_linear_register(const asap_fp8_linear_t* d, uint64_t* handle);
 int asap_fp8_linear_release(uint64_t handle);
 
 /* out [m, n] = x W^T.  x [m, k] bf16 (fp16 != 0: half), rows ldx elements apart (a multiple of 8), 16-byte aligned;
- * out of x's type, rows n apart.  ws: 256-byte aligned scratch of asap_fp8_linear_ws_bytes(m, k), free again when the
- * call's work is done.  A pipeline wait that runs out reports to `status` (0: nowhere). */
+ * out of x's type, rows n apart.  ws: 256-byte aligned scratch of asap_fp8_linear_ws_bytes(m, k) bytes (0: none is
+ * needed, for a few rows; or the arguments are out of range), free again when the call's work is done.  A pipeline wait that runs out reports to `status` (0: nowhere). */
 uint64_t asap_fp8_linear_ws_bytes(int32_t m, int32_t k);
 int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t fp16, uint64_t out, uint64_t ws,
                     uint64_t ws_bytes, uint64_t status, uint64_t timeout_ns, void* stream);

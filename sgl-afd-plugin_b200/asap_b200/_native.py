@@ -183,6 +183,19 @@ def check(name: str, rc: int) -> None:
         raise AsapError(name, rc, msg.decode() if msg else "")
 
 
+_bound: dict = {}
+
+
+def run(name: str, *args) -> None:
+    """call() for calls that come once per operator: the function is looked up once."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(lib(), name)
+    rc = fn(*args)
+    if rc:
+        check(name, rc)
+
+
 def call(name: str, *args) -> int:
     rc = getattr(lib(), name)(*args)
     check(name, rc)

@@ -28,6 +28,7 @@ import torch
 
 from . import _native as N
 
+MAX_ROWS = 1 << 20
 TIMEOUT_NS = 5_000_000_000  # bound of every wait inside the kernels
 _status: dict = {}          # device index -> int64 status word
 
@@ -110,20 +111,21 @@ def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int)
         raise RuntimeError("the layer was released")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != weight.k or x.device != weight.device:
+    if x.dim() < 1 or x.shape[-1] != weight.k or x.get_device() != weight.device.index:
         raise ValueError(f"x must be [..., {weight.k}] on {weight.device}, got {tuple(x.shape)} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the FP8 products have no gradient: call them under torch.no_grad() or detach x")
     shape = (*x.shape[:-1], n)
     rows = x if x.dim() == 2 else x.reshape(-1, weight.k)
-    if rows.shape[0] > 1 << 20:
-        raise ValueError(f"at most {1 << 20} rows per call, got {rows.shape[0]}")
-    ld = rows.stride(0) if rows.shape[0] > 1 else weight.k
-    if (weight.k > 1 and rows.stride(1) != 1) or ld % 8 or ld < weight.k or rows.data_ptr() % 16:
-        rows = rows.clone(memory_format=torch.contiguous_format)
-        ld = weight.k
+    m, ld = rows.shape[0], weight.k
+    if m > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows per call, got {m}")
+    if m > 1 and not rows.is_contiguous():
+        ld = rows.stride(0)
+    if rows.stride(1) != 1 or ld % 8 or ld < weight.k or rows.data_ptr() % 16:
+        rows, ld = rows.clone(memory_format=torch.contiguous_format), weight.k
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
     elif (out.dtype != x.dtype or tuple(out.shape) != shape or out.device != x.device or not out.is_contiguous()
           or out.data_ptr() % 16):
         raise ValueError(f"out must be a contiguous, 16-byte aligned {x.dtype} tensor of shape {shape} on {x.device}")
@@ -131,21 +133,29 @@ def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int)
 
 
 class _OnDevice:
-    """torch.cuda.device(index) that costs nothing when the device is the current one already."""
+    """torch.cuda.device(index), entered only when that is not the current device, -> the device's current
+    raw stream."""
 
-    def __init__(self, device: torch.device):
-        self.index, self.prev = device.index, -1
+    __slots__ = ("index", "prev")
 
-    def __enter__(self):
+    def __init__(self, index: int):
+        self.index, self.prev = index, -1
+
+    def __enter__(self) -> int:
         current = torch.cuda.current_device()
         if current != self.index:
             self.prev = current
             torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.prev >= 0:
             torch.cuda.set_device(self.prev)
         return False
+
+
+def _scratch(nbytes: int, device: torch.device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 class Fp8Linear:
@@ -173,11 +183,10 @@ class Fp8Linear:
         m = rows.shape[0]
         if m:
             nbytes = N.lib().asap_fp8_linear_ws_bytes(m, w.k)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-            with _OnDevice(w.device):
-                N.call("asap_fp8_linear", w.handle, rows.data_ptr(), ld, m, int(x.dtype == torch.float16),
-                       out.data_ptr(), ws.data_ptr(), nbytes, w.status, TIMEOUT_NS,
-                       torch.cuda.current_stream(w.device).cuda_stream)
+            ws = _scratch(nbytes, w.device)
+            with _OnDevice(w.device.index) as stream:
+                N.run("asap_fp8_linear", w.handle, rows.data_ptr(), ld, m, x.dtype == torch.float16, out.data_ptr(),
+                      ws.data_ptr() if nbytes else 0, nbytes, w.status, TIMEOUT_NS, stream)
         return out
 
     def release(self) -> None:
@@ -212,11 +221,10 @@ class Fp8SharedExpert:
         m = rows.shape[0]
         if m:
             nbytes = N.lib().asap_fp8_shared_ws_bytes(m, self.hidden, self.inter)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
-            with _OnDevice(a.device):
-                N.call("asap_fp8_shared", a.handle, b.handle, rows.data_ptr(), ld, m, int(x.dtype == torch.float16),
-                       self.swiglu_limit, out.data_ptr(), ws.data_ptr(), nbytes, a.status, TIMEOUT_NS,
-                       torch.cuda.current_stream(a.device).cuda_stream)
+            ws = _scratch(nbytes, a.device)
+            with _OnDevice(a.device.index) as stream:
+                N.run("asap_fp8_shared", a.handle, b.handle, rows.data_ptr(), ld, m, x.dtype == torch.float16,
+                      self.swiglu_limit, out.data_ptr(), ws.data_ptr(), nbytes, a.status, TIMEOUT_NS, stream)
         return out
 
     def release(self) -> None:

@@ -20,7 +20,6 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .linear import _OnDevice
@@ -56,8 +55,10 @@ def _device_int(name: str, x: torch.Tensor, like: torch.Tensor, shape) -> torch.
     return x.contiguous()
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _once(grad: torch.Tensor) -> None:
+    # backward runs with gradients enabled only under create_graph=True (torch's own guard costs 10 us a call)
+    if torch.is_grad_enabled() and grad.requires_grad:
+        raise RuntimeError("the router's gradients cannot be differentiated again")
 
 
 def _route_forward(logits, opts):
@@ -69,8 +70,8 @@ def _route_forward(logits, opts):
     desc = N.Route_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, k, sigmoid, groups, top_groups, renorm, scale, 0,
                      0 if bias is None else bias.data_ptr(), 0 if num_tokens is None else num_tokens.data_ptr())
     if t:
-        with _OnDevice(rows.device):
-            N.call("asap_route", ctypes.byref(desc), ids.data_ptr(), weights.data_ptr(), _stream(rows.device))
+        with _OnDevice(rows.get_device()) as stream:
+            N.run("asap_route", ctypes.byref(desc), ids.data_ptr(), weights.data_ptr(), stream)
     return weights, ids, rows, desc
 
 
@@ -84,15 +85,14 @@ class _Route(torch.autograd.Function):
         return weights, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_weights, _):
+        _once(grad_weights)
         rows, ids = ctx.saved_tensors
         out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
         if out.numel():
             grad = grad_weights.to(torch.float32).contiguous()
-            with _OnDevice(rows.device):
-                N.call("asap_route_backward", ctypes.byref(ctx.desc), ids.data_ptr(), grad.data_ptr(), out.data_ptr(),
-                       _stream(rows.device))
+            with _OnDevice(rows.get_device()) as stream:
+                N.run("asap_route_backward", ctypes.byref(ctx.desc), ids.data_ptr(), grad.data_ptr(), out.data_ptr(), stream)
         return out, None
 
 
@@ -144,9 +144,8 @@ class _BalanceLoss(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=rows.device)
         desc = N.Balance_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, ids.shape[1], sigmoid, seqs, coef, 0,
                            ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr())
-        with _OnDevice(rows.device):
-            N.call("asap_balance_loss", ctypes.byref(desc), ws.data_ptr(), nbytes, loss.data_ptr(),
-                   _stream(rows.device))
+        with _OnDevice(rows.get_device()) as stream:
+            N.run("asap_balance_loss", ctypes.byref(desc), ws.data_ptr(), nbytes, loss.data_ptr(), stream)
         counts = ws[:seqs * e].view(seqs, e)
         ctx.save_for_backward(rows, ids, ws, *(() if cu_seqlens is None else (cu_seqlens,)))
         ctx.desc, ctx.nbytes = desc, nbytes
@@ -154,14 +153,14 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss, _):
+        _once(grad_loss)
         rows, ids, ws = ctx.saved_tensors[:3]
         out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
         grad = grad_loss.to(torch.float32).contiguous()
-        with _OnDevice(rows.device):
-            N.call("asap_balance_backward", ctypes.byref(ctx.desc), ws.data_ptr(), ctx.nbytes, grad.data_ptr(),
-                   out.data_ptr(), _stream(rows.device))
+        with _OnDevice(rows.get_device()) as stream:
+            N.run("asap_balance_backward", ctypes.byref(ctx.desc), ws.data_ptr(), ctx.nbytes, grad.data_ptr(),
+                   out.data_ptr(), stream)
         return out, None, None, None, None, None
 
 
@@ -208,6 +207,6 @@ def expert_counts(topk_ids: torch.Tensor, num_experts: int) -> torch.Tensor:
         raise ValueError(f"at most {1 << 24} tokens, got {t}")
     ids = topk_ids.contiguous()
     counts = torch.empty(num_experts, dtype=torch.int32, device=ids.device)
-    with _OnDevice(ids.device):
-        N.call("asap_expert_counts", ids.data_ptr(), t, k, num_experts, counts.data_ptr(), _stream(ids.device))
+    with _OnDevice(ids.get_device()) as stream:
+        N.run("asap_expert_counts", ids.data_ptr(), t, k, num_experts, counts.data_ptr(), stream)
     return counts

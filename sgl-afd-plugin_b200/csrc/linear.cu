@@ -191,7 +191,7 @@ static int check_rows(const char* fn, int32_t m, uint64_t x, int64_t ldx, int32_
               (long long)ldx);
     return ASAP_EINVAL;
   }
-  if (!out || (out & 15) || !ws || (ws & 255) || have < need) {
+  if (!out || (out & 15) || (need && (!ws || (ws & 255) || have < need))) {
     set_error("%s: out must be 16-byte and the workspace 256-byte aligned and hold %llu bytes (got %llu)", fn,
               (unsigned long long)need, (unsigned long long)have);
     return ASAP_EINVAL;
@@ -268,6 +268,7 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
 // Up to here the few-rows linear quantises its rows itself.  7168 x 4096: 1 row 10.8 us against 11.0 with a kernel before
 // it (2064 x 1040: 5.3 against 5.8), and one launch less for the caller; 8 rows 13.1 against 11.7.
 constexpr int kInKernelRows = 4;
+constexpr int kInKernelDim = SK_MAX_KB * SK_MAX_SPLIT * BK;  // and this many values of K, whose codes fit the clusters
 
 // How a product of few rows is launched.  rounds: K blocks that a CTA works through, times the waves of clusters.
 struct SkinnyPlan {
@@ -474,6 +475,7 @@ int asap_fp8_linear_release(uint64_t handle) {
 
 uint64_t asap_fp8_linear_ws_bytes(int32_t m, int32_t k) {
   if (m < 1 || m > ASAP_LINEAR_MAX_ROWS || k < 1 || k > ASAP_LINEAR_MAX_DIM) return 0;
+  if (m <= lin::kInKernelRows && k <= lin::kInKernelDim) return 0;
   const lin::ActWs a = lin::act_ws(m, k);
   return a.codes + a.scales;
 }
@@ -492,9 +494,13 @@ int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t
   const lin::ActWs a = lin::act_ws(m, L->d.k);
   lin::SkinnyParams p = lin::skinny_params(x, ldx, m, fp16, a.mp, status, timeout_ns);
   p.out = (void*)out;
-  if (m <= lin::kInKernelRows) {
+  if (m <= lin::kInKernelRows && L->d.k <= lin::kInKernelDim) {
     const lin::SkinnyPlan pl = lin::skinny_plan<0, 0>(L, m);
-    if (pl) return lin::skinny<0, 0>(L, pl, p, 0, 0, st);
+    if (!pl) {
+      set_error("asap_fp8_linear: no launch for %d rows of %d", m, L->d.k);
+      return ASAP_EINVAL;
+    }
+    return lin::skinny<0, 0>(L, pl, p, 0, 0, st);
   }
   const lin::SkinnyPlan pl = lin::skinny_plan<0, 1>(L, m);
   if (pl && pl.rounds < lin::tile_rounds(L, false, m)) {
@@ -506,8 +512,11 @@ int asap_fp8_linear(uint64_t handle, uint64_t x, int64_t ldx, int32_t m, int32_t
 }
 
 uint64_t asap_fp8_shared_ws_bytes(int32_t m, int32_t hidden, int32_t inter) {
-  const uint64_t a = asap_fp8_linear_ws_bytes(m, hidden), b = asap_fp8_linear_ws_bytes(m, inter);
-  return a && b ? a + b : 0;
+  if (m < 1 || m > ASAP_LINEAR_MAX_ROWS || hidden < 1 || hidden > ASAP_LINEAR_MAX_DIM || inter < 1 ||
+      inter > ASAP_LINEAR_MAX_DIM)
+    return 0;
+  const lin::ActWs a = lin::act_ws(m, hidden), b = lin::act_ws(m, inter);
+  return a.codes + a.scales + b.codes + b.scales;
 }
 
 int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t ldx, int32_t m, int32_t fp16,

@@ -156,14 +156,11 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
   const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
   return (uint64_t)hi << 32 | lo;
 }
+// (a, b) becomes the two largest of a >= b and x
 template <typename K>
 __device__ __forceinline__ void top2(K& a, K& b, K x) {
-  if (x > a) {
-    b = a;
-    a = x;
-  } else if (x > b) {
-    b = x;
-  }
+  b = x > a ? a : x > b ? x : b;
+  a = x > a ? x : a;
 }
 
 struct Args {
@@ -181,23 +178,42 @@ struct Args {
 // With groups, only experts of the top_groups best groups take part; a group counts its best key, or with `pairs` the
 // sum of its two best values (one value if it has one).  tol > 0: returns true when two values that had to be compared
 // lie within tol * (1 + |value|) of each other, so the order may differ from that of unrounded scores.
+//
+// Every round takes the warp's best key (one redux), and the lane that held it moves on to its next best.  A lane keeps
+// its two best at hand and goes through its V keys again only when it has given both.
 template <int V, typename S, typename K>
 __device__ __forceinline__ bool select(const Args& p, const K (&key)[V], uint32_t open, bool pairs, S tol, int lane,
                                        int& my_id) {
   bool close = false;
+  K best, second;
+  int at, at2;
+  auto scan = [&] {
+    best = second = 0;
+    at = at2 = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const K x = (open >> i) & 1u ? key[i] : (K)0;
+      const bool b1 = x > best, b2 = x > second;  // strict: the lower index of equal keys comes first
+      second = b1 ? best : b2 ? x : second;
+      at2 = b1 ? at : b2 ? i : at2;
+      best = b1 ? x : best;
+      at = b1 ? i : at;
+    }
+  };
+  scan();
   if (p.groups > 1) {
     const int size = p.e / p.groups, lanes = size / V;
-    K best = 0, second = 0, score = 0;
+    K gbest = 0, gsecond = 0;
     if (size % V == 0 && (lanes & (lanes - 1)) == 0) {  // a group is an aligned run of lanes
-#pragma unroll
-      for (int i = 0; i < V; ++i) top2(best, second, (open >> i) & 1u ? key[i] : (K)0);
+      gbest = best;
+      gsecond = second;
       for (int o = 1; o < lanes; o <<= 1) {
-        const K ob = __shfl_xor_sync(0xffffffffu, best, o), os = __shfl_xor_sync(0xffffffffu, second, o);
-        top2(best, second, ob);
-        top2(best, second, os);
+        const K ob = __shfl_xor_sync(0xffffffffu, gbest, o), os = __shfl_xor_sync(0xffffffffu, gsecond, o);
+        top2(gbest, gsecond, ob);
+        top2(gbest, gsecond, os);
       }
-      best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
-      second = __shfl_sync(0xffffffffu, second, lane * lanes);
+      gbest = __shfl_sync(0xffffffffu, gbest, lane * lanes);  // lane g: group g (lanes >= groups: unused)
+      gsecond = __shfl_sync(0xffffffffu, gsecond, lane * lanes);
     } else {
       for (int g = 0; g < p.groups; ++g) {
         K a = 0, b = 0;
@@ -210,66 +226,97 @@ __device__ __forceinline__ bool select(const Args& p, const K (&key)[V], uint32_
         const uint32_t holders = __ballot_sync(0xffffffffu, a == m);
         const K rest = warp_max(a == m && lane == __ffs(holders) - 1 ? b : a);
         if (lane == g) {
-          best = m;
-          second = rest;
+          gbest = m;
+          gsecond = rest;
         }
       }
     }
-    if (lane < p.groups && best)
-      score = pairs ? key_of(value_of(best) + (second ? value_of(second) : (S)0)) : best;
+    const S ninf = -(S)INFINITY;
+    const bool mine = lane < p.groups && gbest;
+    const S score = !mine ? ninf : pairs ? value_of(gbest) + (gsecond ? value_of(gsecond) : (S)0) : value_of(gbest);
+    const S margin = tol * ((S)1 + (S)fabs(score));
     int rank = 0;
     for (int g = 0; g < p.groups; ++g) {
-      const K o = __shfl_sync(0xffffffffu, score, g);
+      const S o = __shfl_sync(0xffffffffu, score, g);
       rank += o > score || (o == score && g < lane);
-      if (tol > 0 && g != lane && o && score) {
-        const S d = value_of(o) - value_of(score);
-        close |= fabs(d) < tol * ((S)1 + fabs(value_of(o)));
-      }
+      if (tol > 0) close |= g != lane && fabs(o - score) < margin;  // infinite or NaN for a closed group: not close
     }
-    const uint32_t kept = __ballot_sync(0xffffffffu, lane < p.groups && score && rank < p.top_groups);
+    close &= mine;
+    const uint32_t kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
+    if (size % V == 0) {  // one group to a lane
+      if (lane * V < p.e && !((kept >> (lane * V / size)) & 1u)) open = 0, best = second = 0;
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
+      for (int i = 0; i < V; ++i) {
+        const int e = lane * V + i;
+        if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
+      }
+      scan();
     }
   }
-  K best = 0;
-  int at = 0;
-  auto rescan = [&] {
-    best = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (((open >> i) & 1u) && key[i] > best) {
-        best = key[i];
-        at = i;
-      }
-  };
-  rescan();
   my_id = -1;
   K prev = 0;
   const int rounds = tol > 0 ? p.k + 1 : p.k;  // the last one only compares the (k+1)-th with the k-th
   for (int j = 0; j < rounds; ++j) {
     const K m = warp_max(best);
     if (!m) break;
-    if (tol > 0 && j > 0) close |= value_of(prev) - value_of(m) < tol * ((S)1 + fabs(value_of(m)));
+    if (tol > 0 && j > 0) close |= value_of(prev) - value_of(m) < tol * ((S)1 + (S)fabs(value_of(m)));
     const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
     const int id = __shfl_sync(0xffffffffu, lane * V + at, src);
     if (lane == j && j < p.k) my_id = id;
     if (lane == src) {
       open &= ~(1u << at);
-      rescan();
+      best = second;
+      at = at2;
+      second = 0;
+      if (!best && open) scan();
     }
     prev = m;
   }
   return __any_sync(0xffffffffu, close);
 }
 
+// The choice of one row by score + bias in 64 bits, from memory: called for few rows, and kept out of the kernel's
+// registers.
+template <int V>
+__device__ __noinline__ int select_exactly(const Args& p, const void* row, int lane) {
+  const float ninf = __uint_as_float(0xff800000u);
+  float l[V], b[V];
+  load_row<V>(row, p.e, p.dtype, false, lane, ninf, l);
+  load_row<V>(p.bias, p.e, kF32, false, lane, ninf, b);
+  float top = ninf;
+#pragma unroll
+  for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+  top = warp_max(top);
+  double z = 0.0;
+  if (!p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (l[i] > ninf) z += exp((double)l[i] - (double)top);
+    z = warp_sum(z);
+  }
+  uint64_t key[V];
+  uint32_t open = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const double s = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)top) / z;
+    const double x = s + (double)b[i];
+    if (l[i] > ninf && x != -(double)INFINITY) open |= 1u << i;
+    key[i] = x != x ? 1ull : key_of(x);
+  }
+  int id;
+  select<V, double>(p, key, open, true, 0.0, lane, id);
+  return id;
+}
+
 // Without a bias the scores rank as the logits do, so the selection compares logits, exactly.  With one it compares
 // score + bias: first in fp32; a row with two candidates closer than the fp32 error (a few in 10^5 rows) is ranked again
-// in 64 bits.  The bound: |score| <= 1 carries at most 2 * 10^-6 (exp within 2 ulp, a sum of up to 1024 terms, one
-// division, one sum), twice that between two of them.
+// in 64 bits.  The bound: |score| <= 1 carries at most 2 * 10^-6 (exp within 2 ulp, a sum of up to 1024 terms, an
+// approximate division within 2 ulp, one sum), twice that between two of them.
+//
+// Bound by issue slots: some 600 instructions of a warp per token (8 exponentials and divisions per lane, 9 rounds).
 template <int V>
-__global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) route_kernel(const __grid_constant__ Args p) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= p.t) return;
@@ -313,31 +360,16 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constan
     select<V, float>(p, key, open, false, 0.f, lane, id);
   } else {
     float b[V];
+    const float rz = 1.f / z;
     load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float s = p.sigmoid ? 1.f / (1.f + expf(-l[i])) : expf(l[i] - top) / z;
+      const float s = p.sigmoid ? __fdividef(1.f, 1.f + expf(-l[i])) : expf(l[i] - top) * rz;
       const float x = s + b[i];
       if (x == ninf) open &= ~(1u << i);
       key[i] = x != x ? 1u : key_of(x);
     }
-    if (select<V, float>(p, key, open, true, 4e-6f, lane, id)) {
-      double zd = 0.0;
-      if (!p.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if ((open >> i) & 1u) zd += exp((double)l[i] - (double)top);
-        zd = warp_sum(zd);
-      }
-      uint64_t wide[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const double s = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)top) / zd;
-        const double x = s + (double)b[i];
-        wide[i] = x != x ? 1ull : key_of(x);
-      }
-      select<V, double>(p, wide, open, true, 0.0, lane, id);
-    }
+    if (select<V, float>(p, key, open, true, 4e-6f, lane, id)) id = select_exactly<V>(p, row, lane);
   }
   float s = 0.f;
   if (id >= 0) {
@@ -474,63 +506,94 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int seqs, int64_t t) {
   return lo < seqs ? lo : -1;
 }
 
-constexpr int kCountRows = 128;  // tokens per block, one per thread
-__global__ void __launch_bounds__(kCountRows) balance_count_kernel(const __grid_constant__ BalanceArgs p) {
+constexpr int kCountRows = 64;  // tokens per block: their ids are read four to a thread and more
+constexpr int kCountThreads = 128;
+__global__ void __launch_bounds__(kCountThreads) balance_count_kernel(const __grid_constant__ BalanceArgs p) {
   extern __shared__ int32_t hist[];  // the counts of the block's first sequence; [e] = its live tokens
-  for (int i = threadIdx.x; i <= p.e; i += kCountRows) hist[i] = 0;
-  const int64_t t0 = (int64_t)blockIdx.x * kCountRows, t = t0 + threadIdx.x;
+  for (int i = threadIdx.x; i <= p.e; i += kCountThreads) hist[i] = 0;
+  const int64_t t0 = (int64_t)blockIdx.x * kCountRows;
   const int first = seq_of(p.cu, p.seqs, t0);
+  const int n = (int)min((int64_t)kCountRows, p.t - t0) * p.k;
+  const int32_t* ids = p.ids + t0 * p.k;
   __syncthreads();
-  const int s = t < p.t ? seq_of(p.cu, p.seqs, t) : -1;
-  if (s >= 0) {
-    const int32_t* ids = p.ids + t * p.k;
-    bool any = false;
-    for (int j = 0; j < p.k; ++j) {
-      const int e = ids[j];
-      if (e < 0 || e >= p.e) continue;
-      any = true;
-      atomicAdd(s == first ? &hist[e] : &p.counts[(int64_t)s * p.e + e], 1);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += kCountThreads) {
+    const int e = ids[i], r = i / p.k, j = i - r * p.k;
+    const bool valid = e >= 0 && e < p.e;
+    bool live = false;  // the token's first id speaks for the token
+    if (j == 0 && p.live) {
+      live = valid;
+      for (int o = 1; !live && o < p.k; ++o) live = ids[i + o] >= 0 && ids[i + o] < p.e;
     }
-    if (any && p.live) atomicAdd(s == first ? &hist[p.e] : &p.live[s], 1);
+    if (!valid && !live) continue;
+    const int s = p.cu ? seq_of(p.cu, p.seqs, t0 + r) : 0;
+    if (s < 0) continue;
+    if (valid) atomicAdd(s == first ? &hist[e] : &p.counts[(int64_t)s * p.e + e], 1);
+    if (live) atomicAdd(s == first ? &hist[p.e] : &p.live[s], 1);
   }
   __syncthreads();
   if (first < 0) return;
-  for (int i = threadIdx.x; i <= p.e; i += kCountRows)
+  for (int i = threadIdx.x; i <= p.e; i += kCountThreads)
     if (hist[i]) {
       if (i < p.e) atomicAdd(&p.counts[(int64_t)first * p.e + i], hist[i]);
       else if (p.live) atomicAdd(&p.live[first], hist[i]);
     }
 }
 
-// p_e of a row.  With sigmoids a row whose largest logit is negative is scaled by e^-top, so that its values do not
-// underflow before they are normalised.
+// p_e of a row, and q_e = 1 - sigmoid(l_e) with sigmoids.  A row of sigmoids whose largest logit is negative is scaled by
+// e^-top, so that its values do not underflow before they are normalised.
 template <int V>
-__device__ __forceinline__ void row_probabilities(bool sigmoid, float (&l)[V], float (&p)[V]) {
+__device__ __forceinline__ void row_probabilities(bool sigmoid, float (&l)[V], float (&p)[V], float (&q)[V]) {
   const float ninf = __uint_as_float(0xff800000u);
   float top = ninf, z = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
   top = warp_max(top);
+  if (!sigmoid) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (l[i] == ninf) p[i] = 0.f;
-    else if (!sigmoid) p[i] = expf(l[i] - top);
-    else if (top >= 0.f) p[i] = 1.f / (1.f + expf(-l[i]));
-    else p[i] = expf(l[i] - top) / (1.f + expf(l[i]));
-    z += p[i];
+    for (int i = 0; i < V; ++i) p[i] = l[i] == ninf ? 0.f : expf(l[i] - top);
+  } else if (top >= 0.f) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = fminf(expf(-l[i]), 1e30f);  // sigmoid = 1 / (1 + x), 1 - sigmoid = x / (1 + x)
+      const float s = __fdividef(1.f, 1.f + x);
+      p[i] = l[i] == ninf ? 0.f : l[i] != l[i] ? l[i] : s;
+      q[i] = x * s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      q[i] = __fdividef(1.f, 1.f + expf(l[i]));
+      p[i] = l[i] == ninf ? 0.f : expf(l[i] - top) * q[i];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) z += p[i];
   z = warp_sum(z);
   const float r = z > 0.f ? 1.f / z : (z != z ? z : 0.f);
 #pragma unroll
   for (int i = 0; i < V; ++i) p[i] *= r;
 }
 
+// A warp takes a run of tokens, so that the sequence it is in, and that sequence's a_e, change rarely; the next token's
+// logits are on their way while one is worked on.
 template <int V, bool BACK>
-__global__ void __launch_bounds__(32 * kWarps) balance_kernel(const __grid_constant__ BalanceArgs p) {
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(const __grid_constant__ BalanceArgs p) {
   __shared__ int s_filled[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int size = p.dtype == kF32 ? 4 : 2;
+  const float ninf = __uint_as_float(0xff800000u);
+  const int64_t per_warp = (p.t + (int64_t)gridDim.x * kWarps - 1) / ((int64_t)gridDim.x * kWarps);
+  const int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * per_warp, t1 = min((int64_t)p.t, t0 + per_warp);
+  auto row = [&](int64_t t) { return reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * size; };
+  float next[V];
+  int next_id = -1;
+  if (t0 < t1) {
+    load_row<V>(row(t0), p.e, p.dtype, p.vec, lane, ninf, next);
+    if (lane < p.k) next_id = p.ids[t0 * p.k + lane];
+  }
   int filled = 0;
   for (int s = threadIdx.x; s < p.seqs; s += 32 * kWarps) filled += p.live[s] > 0;
   filled = __reduce_add_sync(0xffffffffu, filled);
@@ -540,33 +603,41 @@ __global__ void __launch_bounds__(32 * kWarps) balance_kernel(const __grid_const
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) filled += s_filled[w];
   const float base = p.coef / (float)max(filled, 1) * ((float)p.e / (float)p.k) * (BACK ? *p.grad : 1.f);
-  const int size = p.dtype == kF32 ? 4 : 2;
-  const float ninf = __uint_as_float(0xff800000u);
   double sum = 0.0;
-  for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < p.t; t += (int64_t)gridDim.x * kWarps) {
-    const int s = seq_of(p.cu, p.seqs, t);
-    const int id = lane < p.k ? p.ids[t * p.k + lane] : -1;
-    const bool live = __any_sync(0xffffffffu, id >= 0 && id < p.e) && s >= 0;
-    float d[V];
-    if (live) {
-      float l[V], pr[V];
-      load_row<V>(reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * size, p.e, p.dtype, p.vec, lane, ninf, l);
-      row_probabilities<V>(p.sigmoid != 0, l, pr);
-      const float n = (float)p.live[s];
-      const float a = base / (n * n);
-      const int32_t* counts = p.counts + (int64_t)s * p.e + lane * V;
-      float dot = 0.f;
+  int seq = -1;
+  int64_t seq_end = -1;  // the first token behind `seq`; -1: not looked up
+  float a[V];
+  for (int64_t t = t0; t < t1; ++t) {
+    float l[V];
+    const int id = next_id;
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] = next[i];
+    if (t + 1 < t1) {
+      load_row<V>(row(t + 1), p.e, p.dtype, p.vec, lane, ninf, next);
+      if (lane < p.k) next_id = p.ids[(t + 1) * p.k + lane];
+    }
+    if (t >= seq_end) {
+      seq = seq_of(p.cu, p.seqs, t);
+      seq_end = seq < 0 ? t + 1 : p.cu ? p.cu[seq + 1] : p.t;
+      const float n = seq < 0 ? 1.f : (float)max(p.live[seq], 1);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        d[i] = lane * V + i < p.e ? a * (float)counts[i] : 0.f;
-        dot += d[i] * pr[i];
+        const int e = lane * V + i;
+        a[i] = seq >= 0 && e < p.e ? base / (n * n) * (float)p.counts[(int64_t)seq * p.e + e] : 0.f;
       }
+    }
+    float d[V];
+    if (__any_sync(0xffffffffu, id >= 0 && id < p.e) && seq >= 0) {
+      float pr[V], q[V], dot = 0.f;
+      row_probabilities<V>(p.sigmoid != 0, l, pr, q);
+#pragma unroll
+      for (int i = 0; i < V; ++i) dot += a[i] * pr[i];
       dot = warp_sum(dot);
       if constexpr (BACK) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          d[i] = pr[i] * (d[i] - dot);
-          if (p.sigmoid) d[i] *= 1.f / (1.f + expf(l[i]));
+          d[i] = pr[i] * (a[i] - dot);
+          if (p.sigmoid) d[i] *= q[i];
         }
       } else {
         sum += (double)dot;
@@ -657,11 +728,11 @@ static BalanceWs balance_ws(int64_t seqs, int64_t e) {
   w.ticket = w.live + 4 * seqs;
   w.zeroed = w.ticket + 4;
   w.partial = align_up(w.zeroed, 8);
-  w.bytes = w.partial + 8ull * 8 * sm_count();
+  w.bytes = w.partial + 8ull * 4 * sm_count();
   return w;
 }
 static int balance_grid(int32_t t) {
-  const int64_t blocks = ((int64_t)t + kWarps - 1) / kWarps, cap = 8ll * sm_count();
+  const int64_t blocks = ((int64_t)t + kWarps - 1) / kWarps, cap = 4ll * sm_count();
   return (int)(blocks < cap ? blocks : cap);
 }
 
@@ -792,8 +863,8 @@ int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, u
   a.loss = (float*)loss;
   cudaStream_t st = (cudaStream_t)stream;
   ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->seqs, b->e).zeroed, st));
-  route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountRows, 4 * (b->e + 1),
-                                st>>>(a);
+  route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountThreads,
+                                4 * (b->e + 1), st>>>(a);
   ASAP_CHECK_LAUNCH("balance_count_kernel");
   route::by_experts<route::Loss>(b->e, a, route::balance_grid(b->t), st);
   ASAP_CHECK_LAUNCH("balance_kernel");
@@ -832,7 +903,8 @@ int asap_expert_counts(uint64_t ids, int32_t t, int32_t k, int32_t e, uint64_t c
   a.counts = (int32_t*)counts;
   cudaStream_t st = (cudaStream_t)stream;
   ASAP_CUDA(cudaMemsetAsync((void*)counts, 0, 4ull * e, st));
-  route::balance_count_kernel<<<(t + route::kCountRows - 1) / route::kCountRows, route::kCountRows, 4 * (e + 1), st>>>(a);
+  route::balance_count_kernel<<<(t + route::kCountRows - 1) / route::kCountRows, route::kCountThreads,
+                                4 * (e + 1), st>>>(a);
   ASAP_CHECK_LAUNCH("balance_count_kernel");
   return ASAP_OK;
 }
