@@ -414,7 +414,7 @@ typedef struct {
   int32_t pad;
   uint64_t ids, cu_seqlens;
 } asap_balance_t;
-uint64_t asap_balance_ws_bytes(int32_t seqs, int32_t e);
+uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs, int32_t e);
 int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream);
 int asap_balance_backward(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t grad_loss,
                           uint64_t grad_logits, void* stream);

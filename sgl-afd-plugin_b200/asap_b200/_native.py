@@ -146,7 +146,7 @@ _SIGS = {
                                   c_uint64, c_void_p]),
     "asap_route": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_void_p]),
     "asap_route_backward": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_uint64, c_void_p]),
-    "asap_balance_ws_bytes": (c_uint64, [c_int32, c_int32]),
+    "asap_balance_ws_bytes": (c_uint64, [c_int32, c_int32, c_int32]),
     "asap_balance_loss": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_void_p]),
     "asap_balance_backward": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_uint64, c_void_p]),
     "asap_expert_counts": (c_int32, [c_uint64, c_int32, c_int32, c_int32, c_uint64, c_void_p]),

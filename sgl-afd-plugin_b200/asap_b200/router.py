@@ -139,7 +139,7 @@ class _BalanceLoss(torch.autograd.Function):
     def forward(ctx, logits, ids, sigmoid, coef, cu_seqlens, seqs):
         rows, ld = _rows(logits)
         t, e = rows.shape
-        nbytes = N.lib().asap_balance_ws_bytes(seqs, e)
+        nbytes = N.lib().asap_balance_ws_bytes(t, seqs, e)
         ws = torch.empty((nbytes + 3) // 4, dtype=torch.int32, device=rows.device)
         loss = torch.empty((), dtype=torch.float32, device=rows.device)
         desc = N.Balance_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, ids.shape[1], sigmoid, seqs, coef, 0,

@@ -156,17 +156,11 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
   const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
   return (uint64_t)hi << 32 | lo;
 }
-// (a, b) becomes the two largest of a >= b and x
-template <typename K>
-__device__ __forceinline__ void top2(K& a, K& b, K x) {
-  b = x > a ? a : x > b ? x : b;
-  a = x > a ? x : a;
-}
-
 struct Args {
   const void* logits;
   int64_t ld;
   int32_t dtype, t, e, k, sigmoid, groups, top_groups, renorm, vec;
+  int32_t aligned_groups;  // a group is a whole number of lanes, a power of two of them (or there is one group)
   float scale;
   const float* bias;         // NULL: none
   const int32_t* num_tokens;  // NULL: t
@@ -174,122 +168,109 @@ struct Args {
   float* weights;
 };
 
-// The k best open keys of the warp's row, best first, ties to the lowest expert: lane j gets the j-th expert's id or -1.
-// With groups, only experts of the top_groups best groups take part; a group counts its best key, or with `pairs` the
-// sum of its two best values (one value if it has one).  tol > 0: returns true when two values that had to be compared
-// lie within tol * (1 + |value|) of each other, so the order may differ from that of unrounded scores.
+// ---- the choice, fast form.  A lane sorts its V keys (a Batcher network of min / max); the low bits of a key give way
+// to the expert's place in the lane, so that no index has to be carried along.  Every round takes the warp's best key (one
+// redux) and the lane that held it moves on to its next.
 //
-// Every round takes the warp's best key (one redux), and the lane that held it moves on to its next best.  A lane keeps
-// its two best at hand and goes through its V keys again only when it has given both.
-template <int V, typename S, typename K>
-__device__ __forceinline__ bool select(const Args& p, const K (&key)[V], uint32_t open, bool pairs, S tol, int lane,
+// Keys rank as floats do.  Half-precision logits lose nothing to the place bits, and equal ones are a true tie.  Otherwise
+// two keys that had to be compared and lie within the rounding of the scores, or differ in no bit that is left, make the
+// function return true: the order may differ from that of unrounded scores, and the row has to be ranked exactly.
+template <int V>
+struct Place {
+  static constexpr uint32_t MASK = V - 1;
+};
+
+template <int V>
+__device__ __forceinline__ void sort_descending(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p <<= 1)
+#pragma unroll
+    for (int q = p; q > 0; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+}
+
+// key[i]: the key of expert lane * V + i with its place in the low bits, 0 if it is closed.  tol: how far apart two scores
+// must be to be ranked by their keys (0: keys are exact up to the place bits; `ties` says whether equal ones are a tie).
+template <int V>
+__device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], bool pairs, float tol, bool ties, int lane,
                                        int& my_id) {
+  constexpr uint32_t MASK = Place<V>::MASK;
+  const float ninf = __uint_as_float(0xff800000u);
   bool close = false;
-  K best, second;
-  int at, at2;
-  auto scan = [&] {
-    best = second = 0;
-    at = at2 = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const K x = (open >> i) & 1u ? key[i] : (K)0;
-      const bool b1 = x > best, b2 = x > second;  // strict: the lower index of equal keys comes first
-      second = b1 ? best : b2 ? x : second;
-      at2 = b1 ? at : b2 ? i : at2;
-      best = b1 ? x : best;
-      at = b1 ? i : at;
+  sort_descending<V>(key);
+  if (p.groups > 1) {  // a group is an aligned run of lanes
+    const int lanes = p.e / p.groups / V;
+    uint32_t best = key[0], second = V > 1 ? key[V > 1 ? 1 : 0] : 0u;
+    for (int o = 1; o < lanes; o <<= 1) {
+      const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o), os = __shfl_xor_sync(0xffffffffu, second, o);
+      second = max(min(best, ob), max(second, os));
+      best = max(best, ob);
     }
-  };
-  scan();
-  if (p.groups > 1) {
-    const int size = p.e / p.groups, lanes = size / V;
-    K gbest = 0, gsecond = 0;
-    if (size % V == 0 && (lanes & (lanes - 1)) == 0) {  // a group is an aligned run of lanes
-      gbest = best;
-      gsecond = second;
-      for (int o = 1; o < lanes; o <<= 1) {
-        const K ob = __shfl_xor_sync(0xffffffffu, gbest, o), os = __shfl_xor_sync(0xffffffffu, gsecond, o);
-        top2(gbest, gsecond, ob);
-        top2(gbest, gsecond, os);
-      }
-      gbest = __shfl_sync(0xffffffffu, gbest, lane * lanes);  // lane g: group g (lanes >= groups: unused)
-      gsecond = __shfl_sync(0xffffffffu, gsecond, lane * lanes);
-    } else {
-      for (int g = 0; g < p.groups; ++g) {
-        K a = 0, b = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int e = lane * V + i;
-          top2(a, b, ((open >> i) & 1u) && e >= g * size && e < g * size + size ? key[i] : (K)0);
-        }
-        const K m = warp_max(a);
-        const uint32_t holders = __ballot_sync(0xffffffffu, a == m);
-        const K rest = warp_max(a == m && lane == __ffs(holders) - 1 ? b : a);
-        if (lane == g) {
-          gbest = m;
-          gsecond = rest;
-        }
-      }
-    }
-    const S ninf = -(S)INFINITY;
-    const bool mine = lane < p.groups && gbest;
-    const S score = !mine ? ninf : pairs ? value_of(gbest) + (gsecond ? value_of(gsecond) : (S)0) : value_of(gbest);
-    const S margin = tol * ((S)1 + (S)fabs(score));
+    best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
+    second = __shfl_sync(0xffffffffu, second, lane * lanes);
+    const bool mine = lane < p.groups && best;
+    float score = mine ? value_of(best & ~MASK) : ninf;
+    if (pairs && mine && second) score += value_of(second & ~MASK);
+    const float margin = 2.f * tol * (1.f + fabsf(score));
     int rank = 0;
     for (int g = 0; g < p.groups; ++g) {
-      const S o = __shfl_sync(0xffffffffu, score, g);
+      const float o = __shfl_sync(0xffffffffu, score, g);
       rank += o > score || (o == score && g < lane);
-      if (tol > 0) close |= g != lane && fabs(o - score) < margin;  // infinite or NaN for a closed group: not close
+      // (the distance to a closed group is infinite or NaN: not close)
+      close |= g != lane && (tol > 0.f ? fabsf(o - score) < margin : !ties && o == score);
     }
     close &= mine;
     const uint32_t kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
-    if (size % V == 0) {  // one group to a lane
-      if (lane * V < p.e && !((kept >> (lane * V / size)) & 1u)) open = 0, best = second = 0;
-    } else {
+    if (!((kept >> (lane / lanes & 31)) & 1u)) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = lane * V + i;
-        if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
-      }
-      scan();
+      for (int i = 0; i < V; ++i) key[i] = 0;
     }
   }
   my_id = -1;
-  K prev = 0;
-  const int rounds = tol > 0 ? p.k + 1 : p.k;  // the last one only compares the (k+1)-th with the k-th
-  for (int j = 0; j < rounds; ++j) {
-    const K m = warp_max(best);
+  uint32_t prev = 0;
+  for (int j = 0; j <= p.k; ++j) {  // the last round only compares the (k+1)-th with the k-th
+    const uint32_t m = __reduce_max_sync(0xffffffffu, key[0] & ~MASK);
     if (!m) break;
-    if (tol > 0 && j > 0) close |= value_of(prev) - value_of(m) < tol * ((S)1 + (S)fabs(value_of(m)));
-    const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-    const int id = __shfl_sync(0xffffffffu, lane * V + at, src);
-    if (lane == j && j < p.k) my_id = id;
-    if (lane == src) {
-      open &= ~(1u << at);
-      best = second;
-      at = at2;
-      second = 0;
-      if (!best && open) scan();
+    if (j > 0) {
+      const float v = value_of(m);
+      close |= tol > 0.f ? value_of(prev) - v < tol * (1.f + fabsf(v)) : !ties && m == prev;
     }
     prev = m;
+    const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] & ~MASK) == m)) - 1;
+    const int id = src * V + (int)(MASK - (__shfl_sync(0xffffffffu, key[0], src) & MASK));
+    if (lane == j && j < p.k) my_id = id;
+    if (lane == src) {
+#pragma unroll
+      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+      key[V - 1] = 0;
+    }
   }
   return __any_sync(0xffffffffu, close);
 }
 
-// The choice of one row by score + bias in 64 bits, from memory: called for few rows, and kept out of the kernel's
-// registers.
+// ---- the choice of one row in 64 bits, from memory, for any groups: called for few rows, and kept out of the kernel's
+// registers.  A lane goes through its V keys again for every round.
 template <int V>
-__device__ __noinline__ int select_exactly(const Args& p, const void* row, int lane) {
+__device__ __noinline__ int choose_exactly(const Args& p, const void* row, int lane) {
   const float ninf = __uint_as_float(0xff800000u);
+  const bool pairs = p.bias != nullptr;
   float l[V], b[V];
   load_row<V>(row, p.e, p.dtype, false, lane, ninf, l);
-  load_row<V>(p.bias, p.e, kF32, false, lane, ninf, b);
-  float top = ninf;
-#pragma unroll
-  for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-  top = warp_max(top);
+  if (p.bias) load_row<V>(p.bias, p.e, kF32, false, lane, ninf, b);
   double z = 0.0;
-  if (!p.sigmoid) {
+  float top = ninf;
+  if (p.bias && !p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+    top = warp_max(top);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (l[i] > ninf) z += exp((double)l[i] - (double)top);
@@ -299,24 +280,77 @@ __device__ __noinline__ int select_exactly(const Args& p, const void* row, int l
   uint32_t open = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const double s = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)top) / z;
-    const double x = s + (double)b[i];
+    double x = (double)l[i];
+    if (p.bias) x = (p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)top) / z) + (double)b[i];
     if (l[i] > ninf && x != -(double)INFINITY) open |= 1u << i;
     key[i] = x != x ? 1ull : key_of(x);
   }
-  int id;
-  select<V, double>(p, key, open, true, 0.0, lane, id);
-  return id;
+  if (p.groups > 1) {
+    const int size = p.e / p.groups;
+    double score = -(double)INFINITY;  // lane g: group g
+    for (int g = 0; g < p.groups; ++g) {
+      uint64_t a = 0, c = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = lane * V + i;
+        const uint64_t x = ((open >> i) & 1u) && e / size == g ? key[i] : 0ull;
+        c = x > a ? a : x > c ? x : c;
+        a = x > a ? x : a;
+      }
+      const uint64_t m = warp_max(a);
+      const uint32_t holders = __ballot_sync(0xffffffffu, a == m);
+      const uint64_t rest = warp_max(a == m && lane == __ffs(holders) - 1 ? c : a);
+      if (lane == g && m) score = value_of(m) + (pairs && rest ? value_of(rest) : 0.0);
+    }
+    const bool mine = lane < p.groups && score > -(double)INFINITY;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double o = __shfl_sync(0xffffffffu, score, g);
+      rank += o > score || (o == score && g < lane);
+    }
+    const uint32_t kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane * V + i;
+      if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
+    }
+  }
+  int my_id = -1;
+  for (int j = 0; j < p.k; ++j) {
+    uint64_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (((open >> i) & 1u) && key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    const uint64_t m = warp_max(best);
+    if (!m) break;
+    const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
+    const int id = __shfl_sync(0xffffffffu, lane * V + at, src);
+    if (lane == j) my_id = id;
+    if (lane == src) open &= ~(1u << at);
+  }
+  return my_id;
 }
 
-// Without a bias the scores rank as the logits do, so the selection compares logits, exactly.  With one it compares
-// score + bias: first in fp32; a row with two candidates closer than the fp32 error (a few in 10^5 rows) is ranked again
-// in 64 bits.  The bound: |score| <= 1 carries at most 2 * 10^-6 (exp within 2 ulp, a sum of up to 1024 terms, an
-// approximate division within 2 ulp, one sum), twice that between two of them.
+__device__ __forceinline__ float rcp_approx(float x) {  // within 1 ulp; 0 for infinity
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Without a bias the scores rank as the logits do, so the choice compares logits.  With one it compares score + bias in
+// fp32, and ranks a row with two candidates closer than the fp32 error (a few in 10^5 rows) again in 64 bits.  The bound:
+// |score| <= 1 carries at most 2 * 10^-6 (an exponential, a sum of up to 1024 terms, an approximate reciprocal, one sum;
+// the fast exponential's error grows with |x|, where the sigmoid's slope vanishes), twice that between two of them, and V
+// units in the last place go to the place bits.
 //
-// Bound by issue slots: some 600 instructions of a warp per token (8 exponentials and divisions per lane, 9 rounds).
+// Bound by issue slots: some 550 instructions of a warp per token (an exponential and a reciprocal for each of a lane's
+// experts, sorting them, a round of 20 per place).
 template <int V>
-__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) route_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 5 : 2) route_kernel(const __grid_constant__ Args p) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= p.t) return;
@@ -329,48 +363,48 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) route_kernel(cons
     }
     return;
   }
+  constexpr uint32_t MASK = Place<V>::MASK;
   const float ninf = __uint_as_float(0xff800000u);
   const void* row = reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * (p.dtype == kF32 ? 4 : 2);
   float l[V];
   load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, l);
-  uint32_t open = 0;
   bool nan = false;
-  float top = ninf;
+  float top = ninf, z = 1.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    nan |= l[i] != l[i];
-    if (l[i] > ninf) open |= 1u << i;  // false for NaN
-    top = fmaxf(top, l[i]);
-  }
+  for (int i = 0; i < V; ++i) nan |= l[i] != l[i];
   nan = __any_sync(0xffffffffu, nan);
-  float z = 1.f;
   if (!p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
     top = warp_max(top);
     z = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if ((open >> i) & 1u) z += expf(l[i] - top);
+      if (l[i] > ninf) z += expf(l[i] - top);
     z = warp_sum(z);
   }
   int id;
   uint32_t key[V];
-  if (!p.bias) {
+  bool unsure = !p.aligned_groups;
+  if (!unsure) {
+    if (!p.bias) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = key_of(l[i]);
-    select<V, float>(p, key, open, false, 0.f, lane, id);
-  } else {
-    float b[V];
-    const float rz = 1.f / z;
-    load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
+      for (int i = 0; i < V; ++i) key[i] = l[i] > ninf ? (key_of(l[i]) & ~MASK) | (MASK - i) : 0u;  // false for NaN
+      unsure = choose<V>(p, key, false, 0.f, p.dtype != kF32, lane, id);
+    } else {
+      float b[V];
+      const float rz = 1.f / z;
+      load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float s = p.sigmoid ? __fdividef(1.f, 1.f + expf(-l[i])) : expf(l[i] - top) * rz;
-      const float x = s + b[i];
-      if (x == ninf) open &= ~(1u << i);
-      key[i] = x != x ? 1u : key_of(x);
+      for (int i = 0; i < V; ++i) {
+        const float x = (p.sigmoid ? rcp_approx(1.f + __expf(-l[i])) : expf(l[i] - top) * rz) + b[i];
+        const uint32_t k = x == x ? (key_of(x) & ~MASK) | (MASK - i) : MASK + 1 + MASK - i;
+        key[i] = l[i] > ninf && x != ninf ? k : 0u;
+      }
+      unsure = choose<V>(p, key, true, 4e-6f + V * 2.4e-7f, false, lane, id);
     }
-    if (select<V, float>(p, key, open, true, 4e-6f, lane, id)) id = select_exactly<V>(p, row, lane);
   }
+  if (unsure) id = choose_exactly<V>(p, row, lane);
   float s = 0.f;
   if (id >= 0) {
     const float x = load1(row, id, p.dtype);
@@ -486,7 +520,9 @@ struct BalanceArgs {
   const int32_t* cu;   // [seqs + 1], NULL: one sequence of t tokens
   int32_t* counts;     // [seqs, e]
   int32_t* live;       // [seqs]
-  uint32_t* ticket;
+  uint32_t* ticket;    // [2] blocks that have finished counting / adding
+  float* factor;       // [seqs] coef / S' E / (k n_s^2)
+  int32_t* row_seq;    // [t] the sequence of a live token, else -1
   double* partial;     // [grid]
   float* loss;
   const float* grad;   // d loss, scalar
@@ -506,38 +542,69 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int seqs, int64_t t) {
   return lo < seqs ? lo : -1;
 }
 
-constexpr int kCountRows = 64;  // tokens per block: their ids are read four to a thread and more
+constexpr int kCountRows = 64;  // tokens per block
 constexpr int kCountThreads = 128;
+constexpr int kCountSeqs = 1024;  // up to here the offsets are searched in shared memory
+// Counts and live tokens per sequence, each token's sequence (-1: not live) for the passes over the logits, and, by the
+// block that finishes last, the factor of each sequence's counts in a_se.
 __global__ void __launch_bounds__(kCountThreads) balance_count_kernel(const __grid_constant__ BalanceArgs p) {
-  extern __shared__ int32_t hist[];  // the counts of the block's first sequence; [e] = its live tokens
-  for (int i = threadIdx.x; i <= p.e; i += kCountThreads) hist[i] = 0;
+  extern __shared__ int32_t hist[];  // [e + 1]: the counts of the block's first sequence, and its live tokens
+  __shared__ int32_t s_cu[kCountSeqs + 1], s_seq[kCountRows], s_live[kCountRows];
+  __shared__ bool s_last;
+  __shared__ int s_filled;
+  const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * kCountRows;
-  const int first = seq_of(p.cu, p.seqs, t0);
-  const int n = (int)min((int64_t)kCountRows, p.t - t0) * p.k;
+  const int rows = (int)min((int64_t)kCountRows, p.t - t0), n = rows * p.k;
   const int32_t* ids = p.ids + t0 * p.k;
+  for (int i = tid; i <= p.e; i += kCountThreads) hist[i] = 0;
+  const bool staged = p.cu && p.seqs <= kCountSeqs;
+  if (staged)
+    for (int i = tid; i <= p.seqs; i += kCountThreads) s_cu[i] = p.cu[i];
+  if (tid < kCountRows) s_live[tid] = 0;
   __syncthreads();
+  if (tid < rows) s_seq[tid] = seq_of(staged ? s_cu : p.cu, p.seqs, t0 + tid);
+  __syncthreads();
+  const int first = s_seq[0];
 #pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += kCountThreads) {
-    const int e = ids[i], r = i / p.k, j = i - r * p.k;
-    const bool valid = e >= 0 && e < p.e;
-    bool live = false;  // the token's first id speaks for the token
-    if (j == 0 && p.live) {
-      live = valid;
-      for (int o = 1; !live && o < p.k; ++o) live = ids[i + o] >= 0 && ids[i + o] < p.e;
-    }
-    if (!valid && !live) continue;
-    const int s = p.cu ? seq_of(p.cu, p.seqs, t0 + r) : 0;
-    if (s < 0) continue;
-    if (valid) atomicAdd(s == first ? &hist[e] : &p.counts[(int64_t)s * p.e + e], 1);
-    if (live) atomicAdd(s == first ? &hist[p.e] : &p.live[s], 1);
+  for (int i = tid; i < n; i += kCountThreads) {
+    const int e = ids[i], r = i / p.k, s = s_seq[r];
+    if (e < 0 || e >= p.e || s < 0) continue;
+    s_live[r] = 1;
+    atomicAdd(s == first ? &hist[e] : &p.counts[(int64_t)s * p.e + e], 1);
   }
   __syncthreads();
-  if (first < 0) return;
-  for (int i = threadIdx.x; i <= p.e; i += kCountThreads)
-    if (hist[i]) {
-      if (i < p.e) atomicAdd(&p.counts[(int64_t)first * p.e + i], hist[i]);
-      else if (p.live) atomicAdd(&p.live[first], hist[i]);
-    }
+  if (p.live && tid < rows) {
+    const int s = s_live[tid] ? s_seq[tid] : -1;
+    p.row_seq[t0 + tid] = s;
+    if (s >= 0) atomicAdd(s == first ? &hist[p.e] : &p.live[s], 1);
+  }
+  __syncthreads();
+  if (first >= 0)
+    for (int i = tid; i <= p.e; i += kCountThreads)
+      if (hist[i]) {
+        if (i < p.e) atomicAdd(&p.counts[(int64_t)first * p.e + i], hist[i]);
+        else if (p.live) atomicAdd(&p.live[first], hist[i]);
+      }
+  if (!p.live) return;  // counts alone
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    s_last = atomicAdd(&p.ticket[0], 1u) == gridDim.x - 1;
+    s_filled = 0;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  int filled = 0;
+  for (int s = tid; s < p.seqs; s += kCountThreads) filled += __ldcg(&p.live[s]) > 0;
+  filled = __reduce_add_sync(0xffffffffu, filled);
+  if ((tid & 31) == 0) atomicAdd(&s_filled, filled);
+  __syncthreads();
+  const float base = p.coef / (float)max(s_filled, 1) * ((float)p.e / (float)p.k);
+  for (int s = tid; s < p.seqs; s += kCountThreads) {
+    const float live = (float)max(__ldcg(&p.live[s]), 1);
+    p.factor[s] = base / (live * live);
+  }
 }
 
 // p_e of a row, and q_e = 1 - sigmoid(l_e) with sigmoids.  A row of sigmoids whose largest logit is negative is scaled by
@@ -579,7 +646,6 @@ __device__ __forceinline__ void row_probabilities(bool sigmoid, float (&l)[V], f
 // logits are on their way while one is worked on.
 template <int V, bool BACK>
 __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(const __grid_constant__ BalanceArgs p) {
-  __shared__ int s_filled[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -589,45 +655,33 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(co
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * per_warp, t1 = min((int64_t)p.t, t0 + per_warp);
   auto row = [&](int64_t t) { return reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * size; };
   float next[V];
-  int next_id = -1;
+  int next_seq = -1;
   if (t0 < t1) {
     load_row<V>(row(t0), p.e, p.dtype, p.vec, lane, ninf, next);
-    if (lane < p.k) next_id = p.ids[t0 * p.k + lane];
+    next_seq = p.row_seq[t0];
   }
-  int filled = 0;
-  for (int s = threadIdx.x; s < p.seqs; s += 32 * kWarps) filled += p.live[s] > 0;
-  filled = __reduce_add_sync(0xffffffffu, filled);
-  if (lane == 0) s_filled[warp] = filled;
-  __syncthreads();
-  filled = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) filled += s_filled[w];
-  const float base = p.coef / (float)max(filled, 1) * ((float)p.e / (float)p.k) * (BACK ? *p.grad : 1.f);
+  const float grad = BACK ? *p.grad : 1.f;
   double sum = 0.0;
   int seq = -1;
-  int64_t seq_end = -1;  // the first token behind `seq`; -1: not looked up
   float a[V];
   for (int64_t t = t0; t < t1; ++t) {
     float l[V];
-    const int id = next_id;
+    const int s = next_seq;
 #pragma unroll
     for (int i = 0; i < V; ++i) l[i] = next[i];
     if (t + 1 < t1) {
       load_row<V>(row(t + 1), p.e, p.dtype, p.vec, lane, ninf, next);
-      if (lane < p.k) next_id = p.ids[(t + 1) * p.k + lane];
-    }
-    if (t >= seq_end) {
-      seq = seq_of(p.cu, p.seqs, t);
-      seq_end = seq < 0 ? t + 1 : p.cu ? p.cu[seq + 1] : p.t;
-      const float n = seq < 0 ? 1.f : (float)max(p.live[seq], 1);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = lane * V + i;
-        a[i] = seq >= 0 && e < p.e ? base / (n * n) * (float)p.counts[(int64_t)seq * p.e + e] : 0.f;
-      }
+      next_seq = p.row_seq[t + 1];
     }
     float d[V];
-    if (__any_sync(0xffffffffu, id >= 0 && id < p.e) && seq >= 0) {
+    if (s >= 0) {
+      if (s != seq) {
+        seq = s;
+        const float f = p.factor[s] * grad;
+        const int32_t* counts = p.counts + (int64_t)s * p.e + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = lane * V + i < p.e ? f * (float)counts[i] : 0.f;
+      }
       float pr[V], q[V], dot = 0.f;
       row_probabilities<V>(p.sigmoid != 0, l, pr, q);
 #pragma unroll
@@ -658,7 +712,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(co
       for (int w = 0; w < kWarps; ++w) b += s_sum[w];
       p.partial[blockIdx.x] = b;
       __threadfence();
-      s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+      s_last = atomicAdd(&p.ticket[1], 1u) == gridDim.x - 1;
     }
     __syncthreads();
     if (s_last && warp == 0) {
@@ -672,14 +726,21 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(co
 }
 
 // ------------------------------------------------------------------ host side
+static int per_lane(int e) {  // V
+  int v = 1;
+  while (32 * v < e) v *= 2;
+  return v;
+}
 template <template <int> class F, typename A>
 static void by_experts(int e, const A& a, int grid, cudaStream_t st) {
-  if (e <= 32) F<1>::run(a, grid, st);
-  else if (e <= 64) F<2>::run(a, grid, st);
-  else if (e <= 128) F<4>::run(a, grid, st);
-  else if (e <= 256) F<8>::run(a, grid, st);
-  else if (e <= 512) F<16>::run(a, grid, st);
-  else F<32>::run(a, grid, st);
+  switch (per_lane(e)) {
+    case 1: return F<1>::run(a, grid, st);
+    case 2: return F<2>::run(a, grid, st);
+    case 4: return F<4>::run(a, grid, st);
+    case 8: return F<8>::run(a, grid, st);
+    case 16: return F<16>::run(a, grid, st);
+    default: return F<32>::run(a, grid, st);
+  }
 }
 template <int V>
 struct Forward {
@@ -720,14 +781,16 @@ static bool rows_16(uint64_t base, int64_t ld, int32_t dtype) {
 }
 
 struct BalanceWs {
-  uint64_t live, ticket, partial, zeroed, bytes;
+  uint64_t live, ticket, zeroed, factor, row_seq, partial, bytes;
 };
-static BalanceWs balance_ws(int64_t seqs, int64_t e) {
+static BalanceWs balance_ws(int64_t t, int64_t seqs, int64_t e) {
   BalanceWs w;
   w.live = 4 * seqs * e;
   w.ticket = w.live + 4 * seqs;
-  w.zeroed = w.ticket + 4;
-  w.partial = align_up(w.zeroed, 8);
+  w.zeroed = w.ticket + 8;  // counts, live tokens and tickets start at 0
+  w.factor = w.zeroed;
+  w.row_seq = w.factor + 4 * seqs;
+  w.partial = align_up(w.row_seq + 4 * t, 8);
   w.bytes = w.partial + 8ull * 4 * sm_count();
   return w;
 }
@@ -747,7 +810,7 @@ static int balance_args(const char* fn, BalanceArgs& a, const asap_balance_t* b,
     set_error("%s: need ids and 1 to %d sequences (one without offsets), got %d", fn, 1 << 20, b->seqs);
     return ASAP_EINVAL;
   }
-  const BalanceWs w = balance_ws(b->seqs, b->e);
+  const BalanceWs w = balance_ws(b->t, b->seqs, b->e);
   if (!ws || (ws & 7) || ws_bytes < w.bytes) {
     set_error("%s: the workspace must be 8-byte aligned and hold %llu bytes (got %llu)", fn, (unsigned long long)w.bytes,
               (unsigned long long)ws_bytes);
@@ -768,6 +831,8 @@ static int balance_args(const char* fn, BalanceArgs& a, const asap_balance_t* b,
   a.counts = (int32_t*)ws;
   a.live = (int32_t*)(ws + w.live);
   a.ticket = (uint32_t*)(ws + w.ticket);
+  a.factor = (float*)(ws + w.factor);
+  a.row_seq = (int32_t*)(ws + w.row_seq);
   a.partial = (double*)(ws + w.partial);
   return ASAP_OK;
 }
@@ -804,6 +869,8 @@ int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stre
   a.sigmoid = r->sigmoid;
   a.groups = r->top_groups == r->groups ? 1 : r->groups;  // every group kept: no limit
   a.top_groups = r->top_groups;
+  const int v = route::per_lane(r->e), lanes = r->e / a.groups / v;
+  a.aligned_groups = a.groups == 1 || (r->e % (a.groups * v) == 0 && (lanes & (lanes - 1)) == 0);
   a.renorm = r->renormalize;
   a.vec = route::rows_16(r->logits, r->ld, r->dtype);
   a.scale = r->scale;
@@ -848,9 +915,9 @@ int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weigh
   return ASAP_OK;
 }
 
-uint64_t asap_balance_ws_bytes(int32_t seqs, int32_t e) {
-  if (seqs < 1 || seqs > (1 << 20) || e < 1 || e > ASAP_ROUTE_MAX_EXPERTS) return 0;
-  return route::balance_ws(seqs, e).bytes;
+uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs, int32_t e) {
+  if (t < 1 || t > (1 << 24) || seqs < 1 || seqs > (1 << 20) || e < 1 || e > ASAP_ROUTE_MAX_EXPERTS) return 0;
+  return route::balance_ws(t, seqs, e).bytes;
 }
 
 int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream) {
@@ -862,7 +929,7 @@ int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, u
   }
   a.loss = (float*)loss;
   cudaStream_t st = (cudaStream_t)stream;
-  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->seqs, b->e).zeroed, st));
+  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->t, b->seqs, b->e).zeroed, st));
   route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountThreads,
                                 4 * (b->e + 1), st>>>(a);
   ASAP_CHECK_LAUNCH("balance_count_kernel");
