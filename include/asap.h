@@ -380,7 +380,7 @@ int asap_fp8_shared(uint64_t w13_handle, uint64_t w2_handle, uint64_t x, int64_t
  * (fp32 [e]; 0: by score), exactly as unrounded arithmetic ranks them, ties to the lowest expert; with groups > 1 only
  * among the top_groups best of `groups` equal runs of experts (a group's score: its best expert's, or with a bias the
  * sum of its two best).  weight = scale * score [/ (sum of the selected scores + 1e-20)].  An expert whose logit (or
- * bias) is -inf is never chosen; places left over get id -1, weight 0, and so do the rows from *num_tokens (int32 on the
+ * bias) is -inf or NaN is never chosen; places left over get id -1, weight 0, and so do the rows from *num_tokens (int32 on the
  * device; 0: t) on.  A NaN logit counts as -inf and makes the row's weights NaN. */
 #define ASAP_ROUTE_MAX_EXPERTS 1024
 #define ASAP_ROUTE_MAX_TOPK 32

@@ -15,7 +15,8 @@ int sm_count();
 namespace route {
 
 enum DType { kF32 = 0, kBf16 = 1, kF16 = 2 };
-constexpr int kWarps = 8;  // tokens per block
+constexpr int kWarps = 8;         // tokens that a block works on at a time
+constexpr int kRouteBlocks = 4;  // blocks of the router on an SM
 
 __device__ __forceinline__ float to_float(uint16_t b, int dt) {
   if (dt == kBf16) return __uint_as_float((uint32_t)b << 16);
@@ -161,6 +162,7 @@ struct Args {
   int64_t ld;
   int32_t dtype, t, e, k, sigmoid, groups, top_groups, renorm, vec;
   int32_t aligned_groups;  // a group is a whole number of lanes, a power of two of them (or there is one group)
+  int32_t group_log_lanes;
   float scale;
   const float* bias;         // NULL: none
   const int32_t* num_tokens;  // NULL: t
@@ -173,8 +175,10 @@ struct Args {
 // redux) and the lane that held it moves on to its next.
 //
 // Keys rank as floats do.  Half-precision logits lose nothing to the place bits, and equal ones are a true tie.  Otherwise
-// two keys that had to be compared and lie within the rounding of the scores, or differ in no bit that is left, make the
-// function return true: the order may differ from that of unrounded scores, and the row has to be ranked exactly.
+// two keys that had to be compared may lie within the rounding of the scores, or differ in no bit that is left.  Then the
+// scores of those few candidates are computed in 64 bits and ranked again; what that cannot settle makes the function
+// return true, and the row is ranked exactly from the start.  (Both are kept small and rolled: a few rows of a call take
+// them, and then wait for their instructions to be fetched.)
 template <int V>
 struct Place {
   static constexpr uint32_t MASK = V - 1;
@@ -197,17 +201,35 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[V]) {
           }
 }
 
-// key[i]: the key of expert lane * V + i with its place in the low bits, 0 if it is closed.  tol: how far apart two scores
-// must be to be ranked by their keys (0: keys are exact up to the place bits; `ties` says whether equal ones are a tie).
-template <int V>
-__device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], bool pairs, float tol, bool ties, int lane,
-                                       int& my_id) {
+// key[i]: the key of expert lane * V + i with its place in the low bits; at most kClosed if the expert is closed.
+// TIES: keys that differ in their place only are equal, and go to the lowest expert.  Else such keys are close, and so are
+// two scores within tol + |score| (V + 2) 2^-23 of each other: tol for how the scores were computed (0: they are exact), V
+// units in the last place for the place bits, two for the sum with the bias.
+constexpr uint32_t kClosed = 0x007fffffu;  // the key of -inf
+
+// score + bias of one expert (a sigmoid), or its logit, in 64 bits
+__device__ __noinline__ double exact_score(const Args& p, const void* row, int e) {
+  const double x = (double)load1(row, e, p.dtype);
+  return p.bias ? 1.0 / (1.0 + exp(-x)) + (double)p.bias[e] : x;
+}
+
+template <int V, bool TIES>
+__device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const void* row, int lane, int& my_id) {
   constexpr uint32_t MASK = Place<V>::MASK;
+  constexpr float kUlps = (V + 2) * 1.1920929e-7f;
+  const bool pairs = !TIES && p.bias;
   const float ninf = __uint_as_float(0xff800000u);
-  bool close = false;
+  const float tol = !p.bias ? 0.f : p.sigmoid ? 8e-7f : 4e-6f;
+  const bool refinable = p.sigmoid || !p.bias;  // a softmax takes its whole row
+  auto is_close = [&](uint32_t a, uint32_t b, float times) {  // keys a >= b, both open
+    const float x = value_of(a & ~MASK);
+    // (negated: two infinities are close)
+    return tol > 0.f ? !(x - value_of(b & ~MASK) >= times * (tol + fabsf(x) * kUlps)) : (a & ~MASK) == (b & ~MASK);
+  };
+  my_id = -1;
   sort_descending<V>(key);
   if (p.groups > 1) {  // a group is an aligned run of lanes
-    const int lanes = p.e / p.groups / V;
+    const int lanes = 1 << p.group_log_lanes;
     uint32_t best = key[0], second = V > 1 ? key[V > 1 ? 1 : 0] : 0u;
     for (int o = 1; o < lanes; o <<= 1) {
       const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o), os = __shfl_xor_sync(0xffffffffu, second, o);
@@ -216,112 +238,178 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], bool p
     }
     best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
     second = __shfl_sync(0xffffffffu, second, lane * lanes);
-    const bool mine = lane < p.groups && best;
+    const bool mine = lane < p.groups && best > kClosed;
     float score = mine ? value_of(best & ~MASK) : ninf;
-    if (pairs && mine && second) score += value_of(second & ~MASK);
-    const float margin = 2.f * tol * (1.f + fabsf(score));
-    int rank = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const float o = __shfl_sync(0xffffffffu, score, g);
-      rank += o > score || (o == score && g < lane);
-      // (the distance to a closed group is infinite or NaN: not close)
-      close |= g != lane && (tol > 0.f ? fabsf(o - score) < margin : !ties && o == score);
+    if (pairs && mine && second > kClosed) score += value_of(second & ~MASK);
+    uint32_t k = mine ? key_of(score) : 0u, kept = 0, least = 0;
+    for (int r = 0; r < p.top_groups; ++r) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, k);
+      if (!m) break;
+      const int g = __ffs(__ballot_sync(0xffffffffu, k == m)) - 1;
+      kept |= 1u << g;
+      if (lane == g) k = 0;
+      least = m;
     }
-    close &= mine;
-    const uint32_t kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
-    if (!((kept >> (lane / lanes & 31)) & 1u)) {
+    if (!TIES) {  // the least kept score against the best one dropped
+      const uint32_t drop = __reduce_max_sync(0xffffffffu, k);
+      if (drop && is_close(least, drop, 2.f)) {
+        // a lane's two best, in 64 bits, unless the third may be one of them
+        const bool hard = V > 2 && key[V > 2 ? 2 : 0] > kClosed && is_close(key[V > 2 ? 1 : 0], key[V > 2 ? 2 : 0], 1.f);
+        if (!refinable || __any_sync(0xffffffffu, hard)) return true;
+        double a = -(double)INFINITY, b = a;
+#pragma unroll 1
+        for (int i = 0; i < (V > 1 ? 2 : 1); ++i) {
+          const uint32_t x = i ? key[V > 1 ? 1 : 0] : key[0];
+          const double d = x > kClosed ? exact_score(p, row, lane * V + (int)(MASK - (x & MASK))) : -(double)INFINITY;
+          b = d > a ? a : d;
+          a = d > a ? d : a;
+        }
+#pragma unroll 1
+        for (int o = 1; o < lanes; o <<= 1) {
+          const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+          b = fmax(fmin(a, oa), fmax(b, ob));
+          a = fmax(a, oa);
+        }
+        a = __shfl_sync(0xffffffffu, a, lane * lanes);
+        b = __shfl_sync(0xffffffffu, b, lane * lanes);
+        if (pairs && b > -(double)INFINITY) a += b;
+        int rank = 0;
+#pragma unroll 1
+        for (int g = 0; g < p.groups; ++g) {
+          const double o = __shfl_sync(0xffffffffu, a, g);
+          rank += o > a || (o == a && g < lane);
+        }
+        kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
+      }
+    }
+    if (!((kept >> (lane >> p.group_log_lanes)) & 1u)) {
 #pragma unroll
       for (int i = 0; i < V; ++i) key[i] = 0;
     }
   }
-  my_id = -1;
-  uint32_t prev = 0;
-  for (int j = 0; j <= p.k; ++j) {  // the last round only compares the (k+1)-th with the k-th
-    const uint32_t m = __reduce_max_sync(0xffffffffu, key[0] & ~MASK);
-    if (!m) break;
-    if (j > 0) {
-      const float v = value_of(m);
-      close |= tol > 0.f ? value_of(prev) - v < tol * (1.f + fabsf(v)) : !ties && m == prev;
+  // lane j: the key taken in round j.  Beyond the k-th as long as the next one is close to the last.
+  uint32_t mine = 0, prev = 0;
+  int j = 0;
+  for (;; ++j) {
+    uint32_t m;
+    int src, id;
+    if (TIES) {
+      if (j == p.k) break;
+      m = __reduce_max_sync(0xffffffffu, key[0] & ~MASK);
+      src = __ffs(__ballot_sync(0xffffffffu, (key[0] & ~MASK) == m)) - 1;
+      id = src * V + (int)(MASK - (__shfl_sync(0xffffffffu, key[0], src) & MASK));
+    } else {
+      m = __reduce_max_sync(0xffffffffu, key[0]);
+      if (j >= p.k) {
+        if (m <= kClosed || !is_close(prev, m, 1.f)) break;
+        if (j == 32) return true;
+      }
+      src = __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1;
+      id = src * V + (int)(MASK - (m & MASK));
+      prev = m;
     }
-    prev = m;
-    const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] & ~MASK) == m)) - 1;
-    const int id = src * V + (int)(MASK - (__shfl_sync(0xffffffffu, key[0], src) & MASK));
-    if (lane == j && j < p.k) my_id = id;
-    if (lane == src) {
+    if (lane == j) {
+      mine = m;
+      my_id = id;
+    }
+    const bool taken = lane == src;
 #pragma unroll
-      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-      key[V - 1] = 0;
+    for (int i = 0; i + 1 < V; ++i) key[i] = taken ? key[i + 1] : key[i];
+    key[V - 1] = taken ? 0u : key[V - 1];
+  }
+  if (mine <= kClosed) my_id = -1;
+  if (!TIES) {
+    const uint32_t before = __shfl_up_sync(0xffffffffu, mine, 1);
+    if (__any_sync(0xffffffffu, lane > 0 && mine > kClosed && is_close(before, mine, 1.f))) {
+      if (!refinable) return true;
+      const double d = my_id >= 0 ? exact_score(p, row, my_id) : -(double)INFINITY;
+      int rank = 0, sorted = -1;
+#pragma unroll 1
+      for (int s = 0; s < j; ++s) {
+        const double o = __shfl_sync(0xffffffffu, d, s);
+        const int oid = __shfl_sync(0xffffffffu, my_id, s);
+        rank += o > d || (o == d && (unsigned)oid < (unsigned)my_id);  // -1, no expert, ranks last
+      }
+#pragma unroll 1
+      for (int s = 0; s < j; ++s) {
+        const int r = __shfl_sync(0xffffffffu, rank, s), id = __shfl_sync(0xffffffffu, my_id, s);
+        if (r == lane && id >= 0) sorted = id;
+      }
+      my_id = sorted;
     }
   }
-  return __any_sync(0xffffffffu, close);
+  if (lane >= p.k) my_id = -1;
+  return false;
 }
 
-// ---- the choice of one row in 64 bits, from memory, for any groups: called for few rows, and kept out of the kernel's
-// registers.  A lane goes through its V keys again for every round.
+// ---- the choice of one row in 64 bits, from memory, for any groups.  Rolled loops; a lane goes through its keys again for
+// every group and every round.
 template <int V>
 __device__ __noinline__ int choose_exactly(const Args& p, const void* row, int lane) {
-  const float ninf = __uint_as_float(0xff800000u);
-  const bool pairs = p.bias != nullptr;
-  float l[V], b[V];
-  load_row<V>(row, p.e, p.dtype, false, lane, ninf, l);
-  if (p.bias) load_row<V>(p.bias, p.e, kF32, false, lane, ninf, b);
-  double z = 0.0;
-  float top = ninf;
+  const double ninf = -(double)INFINITY;
+  double z = 0.0, top = ninf;
   if (p.bias && !p.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-    top = warp_max(top);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (l[i] > ninf) z += exp((double)l[i] - (double)top);
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        const int e = lane * V + i;
+        const double x = e < p.e ? (double)load1(row, e, p.dtype) : ninf;
+        if (!pass) top = fmax(top, x);
+        else if (x > ninf) z += exp(x - top);
+      }
+      if (!pass)
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
     z = warp_sum(z);
   }
-  uint64_t key[V];
-  uint32_t open = 0;
-#pragma unroll
+  uint64_t key[V];  // 0: closed
+#pragma unroll 1
   for (int i = 0; i < V; ++i) {
-    double x = (double)l[i];
-    if (p.bias) x = (p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)top) / z) + (double)b[i];
-    if (l[i] > ninf && x != -(double)INFINITY) open |= 1u << i;
-    key[i] = x != x ? 1ull : key_of(x);
+    const int e = lane * V + i;
+    double x = e < p.e ? (double)load1(row, e, p.dtype) : ninf;
+    const bool open = x > ninf;  // false for NaN
+    if (p.bias && open) x = (p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / z) + (double)p.bias[e];
+    key[i] = open && x > ninf ? key_of(x) : 0ull;
   }
   if (p.groups > 1) {
     const int size = p.e / p.groups;
-    double score = -(double)INFINITY;  // lane g: group g
+    double score = ninf;  // lane g: group g
+#pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       uint64_t a = 0, c = 0;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < V; ++i) {
         const int e = lane * V + i;
-        const uint64_t x = ((open >> i) & 1u) && e / size == g ? key[i] : 0ull;
+        const uint64_t x = e >= g * size && e < g * size + size ? key[i] : 0ull;
         c = x > a ? a : x > c ? x : c;
         a = x > a ? x : a;
       }
       const uint64_t m = warp_max(a);
       const uint32_t holders = __ballot_sync(0xffffffffu, a == m);
       const uint64_t rest = warp_max(a == m && lane == __ffs(holders) - 1 ? c : a);
-      if (lane == g && m) score = value_of(m) + (pairs && rest ? value_of(rest) : 0.0);
+      if (lane == g && m) score = value_of(m) + (p.bias && rest ? value_of(rest) : 0.0);
     }
-    const bool mine = lane < p.groups && score > -(double)INFINITY;
     int rank = 0;
+#pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
       const double o = __shfl_sync(0xffffffffu, score, g);
       rank += o > score || (o == score && g < lane);
     }
-    const uint32_t kept = __ballot_sync(0xffffffffu, mine && rank < p.top_groups);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      if (e < p.e && !((kept >> (e / size)) & 1u)) open &= ~(1u << i);
-    }
+    const uint32_t kept = __ballot_sync(0xffffffffu, lane < p.groups && score > ninf && rank < p.top_groups);
+#pragma unroll 1
+    for (int i = 0; i < V; ++i)
+      if (lane * V + i < p.e && !((kept >> ((lane * V + i) / size)) & 1u)) key[i] = 0;
   }
   int my_id = -1;
+#pragma unroll 1
   for (int j = 0; j < p.k; ++j) {
     uint64_t best = 0;
     int at = 0;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < V; ++i)
-      if (((open >> i) & 1u) && key[i] > best) {
+      if (key[i] > best) {
         best = key[i];
         at = i;
       }
@@ -330,7 +418,7 @@ __device__ __noinline__ int choose_exactly(const Args& p, const void* row, int l
     const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
     const int id = __shfl_sync(0xffffffffu, lane * V + at, src);
     if (lane == j) my_id = id;
-    if (lane == src) open &= ~(1u << at);
+    if (lane == src) key[at] = 0;
   }
   return my_id;
 }
@@ -341,79 +429,93 @@ __device__ __forceinline__ float rcp_approx(float x) {  // within 1 ulp; 0 for i
   return r;
 }
 
+__device__ __forceinline__ float exp_approx(float x) {  // within 2 + |x| / 2^24 * 1.5 ulp
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
 // Without a bias the scores rank as the logits do, so the choice compares logits.  With one it compares score + bias in
-// fp32, and ranks a row with two candidates closer than the fp32 error (a few in 10^5 rows) again in 64 bits.  The bound:
-// |score| <= 1 carries at most 2 * 10^-6 (an exponential, a sum of up to 1024 terms, an approximate reciprocal, one sum;
-// the fast exponential's error grows with |x|, where the sigmoid's slope vanishes), twice that between two of them, and V
-// units in the last place go to the place bits.
+// fp32, and ranks a row with two candidates closer than the fp32 error (one in a thousand rows) again in 64 bits.  The
+// bounds: a sigmoid is off by at most 4 * 10^-7 (fast exponential 2^-22 + |x| 2^-23.2 relative, times a slope of at most
+// s (1 - s) <= 1/4; a sum; a reciprocal within 1 ulp), a softmax by 2 * 10^-6 (a sum of up to 1024 terms), and a pair by
+// twice that.
 //
 // Bound by issue slots: some 550 instructions of a warp per token (an exponential and a reciprocal for each of a lane's
 // experts, sorting them, a round of 20 per place).
-template <int V>
-__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 5 : 2) route_kernel(const __grid_constant__ Args p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= p.t) return;
-  int32_t* ids = p.ids + t * p.k;
-  float* weights = p.weights + t * p.k;
-  if (p.num_tokens && t >= *p.num_tokens) {
-    if (lane < p.k) {
-      ids[lane] = -1;
-      weights[lane] = 0.f;
-    }
-    return;
-  }
+// TIES: half-precision logits without a bias
+template <int V, bool TIES>
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? kRouteBlocks : 2) route_kernel(const __grid_constant__ Args p) {
   constexpr uint32_t MASK = Place<V>::MASK;
+  const int lane = threadIdx.x & 31;
+  const int step = gridDim.x * kWarps;
   const float ninf = __uint_as_float(0xff800000u);
-  const void* row = reinterpret_cast<const uint8_t*>(p.logits) + t * p.ld * (p.dtype == kF32 ? 4 : 2);
-  float l[V];
-  load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, l);
-  bool nan = false;
-  float top = ninf, z = 1.f;
+  const int n = p.num_tokens ? min(max(*p.num_tokens, 0), p.t) : p.t;
+  auto row_of = [&](int t) {
+    return reinterpret_cast<const void*>(reinterpret_cast<const uint8_t*>(p.logits) +
+                                         (int64_t)t * p.ld * (p.dtype == kF32 ? 4 : 2));
+  };
+  int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  float next[V];
+  if (t < n) load_row<V>(row_of(t), p.e, p.dtype, p.vec, lane, ninf, next);
+  for (; t < p.t; t += step) {
+    int32_t* ids = p.ids + (int64_t)t * p.k;
+    float* weights = p.weights + (int64_t)t * p.k;
+    if (t >= n) {
+      if (lane < p.k) {
+        ids[lane] = -1;
+        weights[lane] = 0.f;
+      }
+      continue;
+    }
+    const void* row = row_of(t);
+    float l[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) nan |= l[i] != l[i];
-  nan = __any_sync(0xffffffffu, nan);
-  if (!p.sigmoid) {
+    for (int i = 0; i < V; ++i) l[i] = next[i];
+    if (t + step < n) load_row<V>(row_of(t + step), p.e, p.dtype, p.vec, lane, ninf, next);
+    bool nan = false;
+    float top = ninf, z = 1.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-    top = warp_max(top);
-    z = 0.f;
+    for (int i = 0; i < V; ++i) nan |= l[i] != l[i];
+    nan = __any_sync(0xffffffffu, nan);
+    if (!p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (l[i] > ninf) z += expf(l[i] - top);
-    z = warp_sum(z);
-  }
-  int id;
-  uint32_t key[V];
-  bool unsure = !p.aligned_groups;
-  if (!unsure) {
-    if (!p.bias) {
+      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+      top = warp_max(top);
+      z = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = l[i] > ninf ? (key_of(l[i]) & ~MASK) | (MASK - i) : 0u;  // false for NaN
-      unsure = choose<V>(p, key, false, 0.f, p.dtype != kF32, lane, id);
-    } else {
+      for (int i = 0; i < V; ++i)
+        if (l[i] > ninf) z += expf(l[i] - top);
+      z = warp_sum(z);
+    }
+    int id;
+    uint32_t key[V];
+    bool unsure = !p.aligned_groups;
+    if (!unsure) {
       float b[V];
       const float rz = 1.f / z;
-      load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
+      if (!TIES && p.bias)
+        load_row<V>(p.bias, p.e, kF32, (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, lane, ninf, b);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float x = (p.sigmoid ? rcp_approx(1.f + __expf(-l[i])) : expf(l[i] - top) * rz) + b[i];
-        const uint32_t k = x == x ? (key_of(x) & ~MASK) | (MASK - i) : MASK + 1 + MASK - i;
-        key[i] = l[i] > ninf && x != ninf ? k : 0u;
+        float x = l[i];
+        if (!TIES && p.bias) x = (p.sigmoid ? rcp_approx(1.f + exp_approx(-x)) : expf(x - top) * rz) + b[i];
+        x = fmaxf(l[i] > ninf ? x : ninf, ninf);  // NaN is closed
+        key[i] = (key_of(x) & ~MASK) | (MASK - i);
       }
-      unsure = choose<V>(p, key, true, 4e-6f + V * 2.4e-7f, false, lane, id);
+      unsure = choose<V, TIES>(p, key, row, lane, id);
     }
-  }
-  if (unsure) id = choose_exactly<V>(p, row, lane);
-  float s = 0.f;
-  if (id >= 0) {
-    const float x = load1(row, id, p.dtype);
-    s = p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - top) / z;
-  }
-  const float sum = p.renorm ? warp_sum(s) + 1e-20f : 1.f;
-  if (lane < p.k) {
-    ids[lane] = id;
-    weights[lane] = nan ? __uint_as_float(0x7fc00000u) : p.scale * (s / sum);
+    if (unsure) id = choose_exactly<V>(p, row, lane);
+    float s = 0.f;
+    if (id >= 0) {
+      const float x = load1(row, id, p.dtype);
+      s = p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - top) / z;
+    }
+    const float sum = p.renorm ? warp_sum(s) + 1e-20f : 1.f;
+    if (lane < p.k) {
+      ids[lane] = id;
+      weights[lane] = nan ? __uint_as_float(0x7fc00000u) : p.scale * (s / sum);
+    }
   }
 }
 
@@ -744,7 +846,10 @@ static void by_experts(int e, const A& a, int grid, cudaStream_t st) {
 }
 template <int V>
 struct Forward {
-  static void run(const Args& a, int grid, cudaStream_t st) { route_kernel<V><<<grid, 32 * kWarps, 0, st>>>(a); }
+  static void run(const Args& a, int grid, cudaStream_t st) {
+    if (!a.bias && a.dtype != kF32) route_kernel<V, true><<<grid, 32 * kWarps, 0, st>>>(a);
+    else route_kernel<V, false><<<grid, 32 * kWarps, 0, st>>>(a);
+  }
 };
 template <int V>
 struct Backward {
@@ -870,6 +975,7 @@ int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stre
   a.groups = r->top_groups == r->groups ? 1 : r->groups;  // every group kept: no limit
   a.top_groups = r->top_groups;
   const int v = route::per_lane(r->e), lanes = r->e / a.groups / v;
+  while ((2 << a.group_log_lanes) <= lanes) ++a.group_log_lanes;
   a.aligned_groups = a.groups == 1 || (r->e % (a.groups * v) == 0 && (lanes & (lanes - 1)) == 0);
   a.renorm = r->renormalize;
   a.vec = route::rows_16(r->logits, r->ld, r->dtype);
@@ -878,7 +984,8 @@ int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stre
   a.num_tokens = (const int32_t*)r->num_tokens;
   a.ids = (int32_t*)ids;
   a.weights = (float*)weights;
-  route::by_experts<route::Forward>(r->e, a, (r->t + route::kWarps - 1) / route::kWarps, (cudaStream_t)stream);
+  const int blocks = (r->t + route::kWarps - 1) / route::kWarps, cap = route::kRouteBlocks * sm_count();
+  route::by_experts<route::Forward>(r->e, a, blocks < cap ? blocks : cap, (cudaStream_t)stream);
   ASAP_CHECK_LAUNCH("route_kernel");
   return ASAP_OK;
 }
