@@ -403,8 +403,8 @@ int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weigh
 /* Balance loss of a choice of experts, per sequence: loss = coef * mean over the sequences with a live token of sum_e
  * f_e P_e, f_e = e / (k n) * count_e, P_e = mean of p_te over the sequence's n live tokens (those with an id), p the
  * row's softmax or its sigmoids normalised to sum 1.  ids int32 [t, k], -1: none.  cu_seqlens int32 [seqs + 1] on the
- * device, from 0, not decreasing (0: one sequence); tokens behind the last sequence do not take part.  The workspace
- * starts with the counts, int32 [seqs, e]; the gradient reads it again.  The loss is the same bits every time. */
+ * device, from 0, not decreasing (0: one sequence); tokens behind the last sequence do not take part.  counts int32
+ * [seqs, e] is written; the gradient reads it and the workspace again.  The loss is the same bits every time. */
 typedef struct {
   uint64_t logits;
   int64_t ld;
@@ -412,9 +412,9 @@ typedef struct {
   int32_t sigmoid, seqs;
   float coef;
   int32_t pad;
-  uint64_t ids, cu_seqlens;
+  uint64_t ids, cu_seqlens, counts;
 } asap_balance_t;
-uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs, int32_t e);
+uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs);
 int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream);
 int asap_balance_backward(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t grad_loss,
                           uint64_t grad_logits, void* stream);

@@ -67,7 +67,7 @@ class Route_t(ctypes.Structure):
 class Balance_t(ctypes.Structure):
     _fields_ = [("logits", c_uint64), ("ld", c_int64), ("dtype", c_int32), ("t", c_int32), ("e", c_int32),
                 ("k", c_int32), ("sigmoid", c_int32), ("seqs", c_int32), ("coef", c_float), ("pad", c_int32),
-                ("ids", c_uint64), ("cu_seqlens", c_uint64)]
+                ("ids", c_uint64), ("cu_seqlens", c_uint64), ("counts", c_uint64)]
 
 
 # name -> (restype, argtypes); every int-returning call is checked
@@ -146,7 +146,7 @@ _SIGS = {
                                   c_uint64, c_void_p]),
     "asap_route": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_void_p]),
     "asap_route_backward": (c_int32, [POINTER(Route_t), c_uint64, c_uint64, c_uint64, c_void_p]),
-    "asap_balance_ws_bytes": (c_uint64, [c_int32, c_int32, c_int32]),
+    "asap_balance_ws_bytes": (c_uint64, [c_int32, c_int32]),
     "asap_balance_loss": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_void_p]),
     "asap_balance_backward": (c_int32, [POINTER(Balance_t), c_uint64, c_uint64, c_uint64, c_uint64, c_void_p]),
     "asap_expert_counts": (c_int32, [c_uint64, c_int32, c_int32, c_int32, c_uint64, c_void_p]),

@@ -88,7 +88,7 @@ class _Route(torch.autograd.Function):
     def backward(ctx, grad_weights, _):
         _once(grad_weights)
         rows, ids = ctx.saved_tensors
-        out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         if out.numel():
             grad = grad_weights.to(torch.float32).contiguous()
             with _OnDevice(rows.get_device()) as stream:
@@ -139,15 +139,15 @@ class _BalanceLoss(torch.autograd.Function):
     def forward(ctx, logits, ids, sigmoid, coef, cu_seqlens, seqs):
         rows, ld = _rows(logits)
         t, e = rows.shape
-        nbytes = N.lib().asap_balance_ws_bytes(t, seqs, e)
-        ws = torch.empty((nbytes + 3) // 4, dtype=torch.int32, device=rows.device)
+        nbytes = N.lib().asap_balance_ws_bytes(t, seqs)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
+        counts = torch.empty((seqs, e), dtype=torch.int32, device=rows.device)
         loss = torch.empty((), dtype=torch.float32, device=rows.device)
         desc = N.Balance_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, ids.shape[1], sigmoid, seqs, coef, 0,
-                           ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr())
+                           ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), counts.data_ptr())
         with _OnDevice(rows.get_device()) as stream:
             N.run("asap_balance_loss", ctypes.byref(desc), ws.data_ptr(), nbytes, loss.data_ptr(), stream)
-        counts = ws[:seqs * e].view(seqs, e)
-        ctx.save_for_backward(rows, ids, ws, *(() if cu_seqlens is None else (cu_seqlens,)))
+        ctx.save_for_backward(rows, ids, ws, counts)
         ctx.desc, ctx.nbytes = desc, nbytes
         ctx.mark_non_differentiable(counts)
         return loss, counts
@@ -155,8 +155,8 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_loss, _):
         _once(grad_loss)
-        rows, ids, ws = ctx.saved_tensors[:3]
-        out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        rows, _, ws, _ = ctx.saved_tensors  # all of them: what changed since is refused
+        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         grad = grad_loss.to(torch.float32).contiguous()
         with _OnDevice(rows.get_device()) as stream:
             N.run("asap_balance_backward", ctypes.byref(ctx.desc), ws.data_ptr(), ctx.nbytes, grad.data_ptr(),

@@ -827,6 +827,83 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(co
   }
 }
 
+// A few tokens in one block and one launch: the counts, sequences and factors as balance_count_kernel leaves them, and the
+// loss.
+constexpr int kSmallWarps = 32, kSmallTokens = 1024, kSmallCounts = 4096;  // tokens; sequences times experts
+template <int V>
+__global__ void __launch_bounds__(32 * kSmallWarps) balance_small_kernel(const __grid_constant__ BalanceArgs p) {
+  __shared__ int32_t s_counts[kSmallCounts], s_live[kSmallCounts], s_seq[kSmallTokens];
+  __shared__ double s_sum[kSmallWarps];
+  __shared__ int s_filled;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int size = p.dtype == kF32 ? 4 : 2;
+  const float ninf = __uint_as_float(0xff800000u);
+  const int cells = p.seqs * p.e;
+  for (int i = tid; i < cells; i += 32 * kSmallWarps) s_counts[i] = 0;
+  for (int i = tid; i < p.seqs; i += 32 * kSmallWarps) s_live[i] = 0;
+  if (tid == 0) s_filled = 0;
+  __syncthreads();
+  for (int t = tid; t < p.t; t += 32 * kSmallWarps) {
+    const int s = seq_of(p.cu, p.seqs, t);
+    bool any = false;
+    if (s >= 0)
+      for (int j = 0; j < p.k; ++j) {
+        const int e = p.ids[(int64_t)t * p.k + j];
+        if (e < 0 || e >= p.e) continue;
+        any = true;
+        atomicAdd(&s_counts[s * p.e + e], 1);
+      }
+    if (any) atomicAdd(&s_live[s], 1);
+    s_seq[t] = any ? s : -1;
+    p.row_seq[t] = any ? s : -1;
+  }
+  __syncthreads();
+  int filled = 0;
+  for (int s = tid; s < p.seqs; s += 32 * kSmallWarps) filled += s_live[s] > 0;
+  filled = __reduce_add_sync(0xffffffffu, filled);
+  if (lane == 0) atomicAdd(&s_filled, filled);
+  __syncthreads();
+  const float base = p.coef / (float)max(s_filled, 1) * ((float)p.e / (float)p.k);
+  for (int s = tid; s < p.seqs; s += 32 * kSmallWarps) {
+    const float live = (float)max(s_live[s], 1);
+    p.factor[s] = base / (live * live);
+    p.live[s] = s_live[s];
+  }
+  for (int i = tid; i < cells; i += 32 * kSmallWarps) p.counts[i] = s_counts[i];
+  double sum = 0.0;
+  constexpr int U = V <= 2 ? 4 : V <= 4 ? 2 : 1;  // rows on their way at once
+  for (int t0 = warp; t0 < p.t; t0 += U * kSmallWarps) {
+    float l[U][V];
+    int seq[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kSmallWarps;
+      seq[u] = t < p.t ? s_seq[t] : -1;
+      if (seq[u] >= 0)
+        load_row<V>(reinterpret_cast<const uint8_t*>(p.logits) + (int64_t)t * p.ld * size, p.e, p.dtype, p.vec, lane, ninf,
+                    l[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (seq[u] < 0) continue;
+      float pr[V], q[V], dot = 0.f;
+      row_probabilities<V>(p.sigmoid != 0, l[u], pr, q);
+      const float live = (float)s_live[seq[u]], f = base / (live * live);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane * V + i < p.e) dot += f * (float)s_counts[seq[u] * p.e + lane * V + i] * pr[i];
+      sum += (double)warp_sum(dot);
+    }
+  }
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    double b = 0.0;
+    for (int w = 0; w < kSmallWarps; ++w) b += s_sum[w];
+    *p.loss = (float)b;
+  }
+}
+
 // ------------------------------------------------------------------ host side
 static int per_lane(int e) {  // V
   int v = 1;
@@ -862,6 +939,10 @@ struct Loss {
   }
 };
 template <int V>
+struct LossSmall {
+  static void run(const BalanceArgs& a, int, cudaStream_t st) { balance_small_kernel<V><<<1, 32 * kSmallWarps, 0, st>>>(a); }
+};
+template <int V>
 struct LossBack {
   static void run(const BalanceArgs& a, int grid, cudaStream_t st) {
     balance_kernel<V, true><<<grid, 32 * kWarps, 0, st>>>(a);
@@ -886,13 +967,12 @@ static bool rows_16(uint64_t base, int64_t ld, int32_t dtype) {
 }
 
 struct BalanceWs {
-  uint64_t live, ticket, zeroed, factor, row_seq, partial, bytes;
+  uint64_t ticket, zeroed, factor, row_seq, partial, bytes;
 };
-static BalanceWs balance_ws(int64_t t, int64_t seqs, int64_t e) {
+static BalanceWs balance_ws(int64_t t, int64_t seqs) {
   BalanceWs w;
-  w.live = 4 * seqs * e;
-  w.ticket = w.live + 4 * seqs;
-  w.zeroed = w.ticket + 8;  // counts, live tokens and tickets start at 0
+  w.ticket = 4 * seqs;     // after the live tokens
+  w.zeroed = w.ticket + 8;  // live tokens and tickets start at 0
   w.factor = w.zeroed;
   w.row_seq = w.factor + 4 * seqs;
   w.partial = align_up(w.row_seq + 4 * t, 8);
@@ -910,12 +990,12 @@ static int balance_args(const char* fn, BalanceArgs& a, const asap_balance_t* b,
     return ASAP_EINVAL;
   }
   if (int rc = check_logits(fn, b->logits, b->ld, b->dtype, b->t, b->e, b->k)) return rc;
-  if (!b->ids || (b->ids & 3) || b->seqs < 1 || b->seqs > (1 << 20) || (!b->cu_seqlens && b->seqs != 1) ||
+  if (!b->counts || (b->counts & 3) || !b->ids || (b->ids & 3) || b->seqs < 1 || b->seqs > (1 << 20) || (!b->cu_seqlens && b->seqs != 1) ||
       (b->cu_seqlens & 3)) {
-    set_error("%s: need ids and 1 to %d sequences (one without offsets), got %d", fn, 1 << 20, b->seqs);
+    set_error("%s: need ids, counts and 1 to %d sequences (one without offsets), got %d", fn, 1 << 20, b->seqs);
     return ASAP_EINVAL;
   }
-  const BalanceWs w = balance_ws(b->t, b->seqs, b->e);
+  const BalanceWs w = balance_ws(b->t, b->seqs);
   if (!ws || (ws & 7) || ws_bytes < w.bytes) {
     set_error("%s: the workspace must be 8-byte aligned and hold %llu bytes (got %llu)", fn, (unsigned long long)w.bytes,
               (unsigned long long)ws_bytes);
@@ -933,8 +1013,8 @@ static int balance_args(const char* fn, BalanceArgs& a, const asap_balance_t* b,
   a.coef = b->coef;
   a.ids = (const int32_t*)b->ids;
   a.cu = (const int32_t*)b->cu_seqlens;
-  a.counts = (int32_t*)ws;
-  a.live = (int32_t*)(ws + w.live);
+  a.counts = (int32_t*)b->counts;
+  a.live = (int32_t*)ws;
   a.ticket = (uint32_t*)(ws + w.ticket);
   a.factor = (float*)(ws + w.factor);
   a.row_seq = (int32_t*)(ws + w.row_seq);
@@ -1022,9 +1102,9 @@ int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weigh
   return ASAP_OK;
 }
 
-uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs, int32_t e) {
-  if (t < 1 || t > (1 << 24) || seqs < 1 || seqs > (1 << 20) || e < 1 || e > ASAP_ROUTE_MAX_EXPERTS) return 0;
-  return route::balance_ws(t, seqs, e).bytes;
+uint64_t asap_balance_ws_bytes(int32_t t, int32_t seqs) {
+  if (t < 1 || t > (1 << 24) || seqs < 1 || seqs > (1 << 20)) return 0;
+  return route::balance_ws(t, seqs).bytes;
 }
 
 int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, uint64_t loss, void* stream) {
@@ -1036,7 +1116,13 @@ int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, u
   }
   a.loss = (float*)loss;
   cudaStream_t st = (cudaStream_t)stream;
-  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->t, b->seqs, b->e).zeroed, st));
+  if ((int64_t)b->t * route::per_lane(b->e) <= route::kSmallTokens && (int64_t)b->seqs * b->e <= route::kSmallCounts) {
+    route::by_experts<route::LossSmall>(b->e, a, 1, st);
+    ASAP_CHECK_LAUNCH("balance_small_kernel");
+    return ASAP_OK;
+  }
+  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->t, b->seqs).zeroed, st));
+  ASAP_CUDA(cudaMemsetAsync((void*)b->counts, 0, 4ull * b->seqs * b->e, st));
   route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountThreads,
                                 4 * (b->e + 1), st>>>(a);
   ASAP_CHECK_LAUNCH("balance_count_kernel");
