@@ -4,11 +4,15 @@ Same API as the reference's python/sgl_asap_plugin/srt/layers/moe/ep_moe/layer.p
 returns ``AsapMoE``, a FusedMoE stand-in without expert weights whose forward hands the routed experts to the
 FFN ranks through ``AsapDispatcher``.  ``should_fuse_routed_scaling_factor_in_topk`` is True (the weights on the
 wire already include the routed scale) and ``quant_method`` is None (layer.py:36-81).
+
+``shared_expert`` (None: as the reference, which adds the shared experts outside) is called on the hidden states between
+dispatch and combine, while the FFN ranks work, and its output is added in the combine kernel: an
+``asap_b200.linear.Fp8SharedExpert``, or any callable of the same shape.
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Callable, Optional
 
 import torch
 
@@ -43,10 +47,13 @@ class AsapMoE(torch.nn.Module):
             params_dtype=params_dtype, inplace=False, routed_scaling_factor=routed_scaling_factor)
         self.dispatcher = AsapDispatcher(layer_id)
         self.shared_experts_overlap = None
+        self.shared_expert: Optional[Callable[[torch.Tensor], torch.Tensor]] = None
 
     def forward(self, hidden_states: torch.Tensor, topk_output, pre_quant_input=None) -> torch.Tensor:
         overlap = self.shared_experts_overlap
         if overlap is not None and getattr(overlap, "active", False):
             overlap.pre_quant_input = pre_quant_input
         dispatch_output = self.dispatcher.dispatch(hidden_states, topk_output)
-        return self.dispatcher.combine(dispatch_output)
+        if self.shared_expert is None:
+            return self.dispatcher.combine(dispatch_output)
+        return self.dispatcher.combine(dispatch_output, shared=self.shared_expert(hidden_states))
