@@ -5,14 +5,19 @@
 // of two and cannot ride in the MMA, so every 128-deep K block is accumulated on its own into one of two TMEM buffers
 // and folded into fp32 registers (one fma per element) while the tensor core fills the other buffer.
 //
-// What bounds it is the turn-around of those two buffers: MMA done -> a folding warp sees it -> two TMEM loads, half
-// the fmas, two more loads -> the MMA issuer sees the buffer free.  A wait on an mbarrier costs about 200 cycles here
-// even when its phase is long over (the MMAs keep shared memory busy), and the issuer used to make three per K block,
-// which alone took 620 of its 1170 cycles.  So a K block has one barrier to start (`ready`: operands and scales
-// landed, buffer free) and one when it is done (`done`: stage free, partial complete).  The activation scales come
-// through the same ring, a K block ahead of the operands (512 bytes per block): when a block is done the next one's
-// scales have landed, and a folding warp reads them while its last fmas run, so that neither a load from memory nor one
-// from shared memory (200 cycles as well) is on the turn-around.
+// What bounds it is the turn-around of those buffers: MMA done -> a folding warp sees it -> two TMEM loads, half the
+// fmas, two more loads -> the MMA issuer sees the buffer free.  A wait on an mbarrier costs about 200 cycles here even
+// when its phase is long over (the MMAs keep shared memory busy), and the issuer used to make three per K block, which
+// alone took 620 of its 1170 cycles.  So:
+// - a K block has one barrier to start (`ready`: operands and scales landed, buffer free) and one when it is done
+//   (`done`: stage free, partial complete), and both sides ask for the next one before they use the answer;
+// - the activation scales come through the same ring, a K block ahead of the operands (512 bytes per block): when a block
+//   is done the next one's scales have landed, and a folding warp reads them while its last fmas run;
+// - a K block is issued as two halves of 128 columns, each with its own barriers and its own four folding warps: one
+//   half's turn-around runs under the other's MMAs.  (Alone, MMAs of 128 columns take 710 cycles per K block, those of
+//   256 take 512; folded, 976 against 1009.)
+// 8192 x 8192 x 7168: 520 us = 1.85 PFLOP/s by itself.  In a row of launches the 1000 W cap sets the clock (1.65 GHz): 612
+// us with the quantisation.
 #pragma once
 
 namespace lin {
@@ -26,7 +31,6 @@ constexpr int SCALE_BYTES = BM * 4;  // a K block's activation scales
 // it + SCALE_SLOTS - 3 - STAGES >= it.
 constexpr int SCALE_SLOTS = 8;
 static_assert(SCALE_SLOTS >= STAGES + 3, "a folding warp may still read the slot");
-constexpr uint32_t STAGE_TX = A_BYTES + B_BYTES;
 constexpr int EPI_WARPS = 8, EPI_BASE = 4, THREADS = 32 * (EPI_BASE + EPI_WARPS);
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int STAGE_OUT_BYTES = EPI_WARPS * 2048;
@@ -174,9 +178,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
   uint8_t* sOut = reinterpret_cast<uint8_t*>(sSa) + SCALE_SLOTS * SCALE_BYTES;
   uint8_t* ctrl = sOut + STAGE_OUT_BYTES;
   // K block `it` uses stage it % STAGES, scale slot it % SCALE_SLOTS and TMEM buffer it % 2
-  uint64_t* ready = reinterpret_cast<uint64_t*>(ctrl);  // [STAGES] operands, scales and buffer: the MMAs may start
-  uint64_t* done = ready + STAGES;                      // [STAGES] the MMAs have completed
-  uint64_t* mma_done = done + STAGES;
+  uint64_t* ready = reinterpret_cast<uint64_t*>(ctrl);  // [STAGES][2 halves] operands, scales, buffer: the MMAs may start
+  uint64_t* done = ready + 2 * STAGES;                  // [STAGES][2] the half's MMAs have completed
+  uint64_t* mma_done = done + 2 * STAGES;
   uint64_t* amax_bar = mma_done + 1;  // [4 lane quarters][2 tile parities]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 516);
@@ -184,8 +188,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&ready[s], 1 + EPI_WARPS);
+    for (int s = 0; s < 2 * STAGES; ++s) {
+      mbar_init(&ready[s], 1 + EPI_WARPS / 2);
       mbar_init(&done[s], 1);
     }
     mbar_init(mma_done, 1);
@@ -225,18 +229,30 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           const float* sa = p.sa + (int64_t)m_t * BM;
           const int b0 = SWIGLU ? n_t * 128 : n_t * BN, b1 = SWIGLU ? p.N / 2 + n_t * 128 : n_t * BN + 128;
           for (int kb = 0; kb < KB; ++kb, ++it) {
-            if (!mbar_wait(&done[stage], phase ^ 1u, deadline, abort_flag)) {
+            // (the second half's commit follows the first's, so it speaks for both)
+            if (!mbar_wait(&done[2 * stage + 1], phase ^ 1u, deadline, abort_flag)) {
               ok = false;
               break;
             }
             const int scales = (kb == 0) + (kb + 1 < KB);
-            mbar_arrive_expect_tx(&ready[stage], STAGE_TX + scales * SCALE_BYTES);
-            tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, kb * BK, m_t * BM, &ready[stage]);
-            tma_load_2d(sB + stage * B_BYTES, &p.tmap_b, kb * BK, b0, &ready[stage]);
-            tma_load_2d(sB + stage * B_BYTES + B_HALF, &p.tmap_b, kb * BK, b1, &ready[stage]);
-            if (kb == 0) bulk_load(sSa + it % SCALE_SLOTS * BM, sa, SCALE_BYTES, &ready[stage]);
+            uint64_t* bar = &ready[2 * stage];
+            uint8_t* b = sB + stage * B_BYTES;
+            mbar_arrive_expect_tx(bar, A_BYTES + B_HALF + scales * SCALE_BYTES);
+            tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, kb * BK, m_t * BM, bar);
+            if (kb == 0) bulk_load(sSa + it % SCALE_SLOTS * BM, sa, SCALE_BYTES, bar);
             if (kb + 1 < KB)
-              bulk_load(sSa + (it + 1) % SCALE_SLOTS * BM, sa + (int64_t)(kb + 1) * p.mp, SCALE_BYTES, &ready[stage]);
+              bulk_load(sSa + (it + 1) % SCALE_SLOTS * BM, sa + (int64_t)(kb + 1) * p.mp, SCALE_BYTES, bar);
+            if constexpr (SWIGLU) {  // boxes of 64 rows: a half holds 64 gate rows and the 64 up rows they meet
+              tma_load_2d(b, &p.tmap_b, kb * BK, b0, bar);
+              tma_load_2d(b + B_HALF / 2, &p.tmap_b, kb * BK, b1, bar);
+              mbar_arrive_expect_tx(bar + 1, B_HALF);
+              tma_load_2d(b + B_HALF, &p.tmap_b, kb * BK, b0 + 64, bar + 1);
+              tma_load_2d(b + B_HALF + B_HALF / 2, &p.tmap_b, kb * BK, b1 + 64, bar + 1);
+            } else {
+              tma_load_2d(b, &p.tmap_b, kb * BK, b0, bar);
+              mbar_arrive_expect_tx(bar + 1, B_HALF);
+              tma_load_2d(b + B_HALF, &p.tmap_b, kb * BK, b1, bar + 1);
+            }
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -246,31 +262,30 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer: one K block per TMEM buffer, alternating.  The warp runs the loop as a whole and one
-      // elected lane issues, so that descriptors stay in uniform registers (1057 -> 1009 cycles per K block).
+      // elected lane issues, so that descriptors stay in uniform registers (5% of a K block's time).
       {
-        int stage = 0;
-        uint32_t phase = 0, it = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-          for (int kb = 0; kb < KB; ++kb, ++it) {
-            const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES), bdesc = sdesc_sw128(sB + stage * B_BYTES);
-            const uint32_t acc = tmem_base + (it & 1u) * BN;
-            ok = __all_sync(0xffffffffu, mbar_wait(&ready[stage], phase, deadline, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
+        // Halves are numbered through: half x is K block x / 2, barrier pair x % (2 STAGES).  Whether the next half may
+        // start is asked before this half's MMAs are issued, and the answer used after.
+        const uint32_t total = (uint32_t)(num_tiles - (int)blockIdx.x + (int)gridDim.x - 1) / gridDim.x * (uint32_t)KB * 2u;
+        bool ok = true, early = false;
+        for (uint32_t x = 0; ok && x < total; ++x) {
+          const uint32_t slot = x % (2 * STAGES), stage = slot / 2, h = x & 1u, next = (x + 1) % (2 * STAGES);
+          const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES);
+          const uint64_t bdesc = sdesc_sw128(sB + stage * B_BYTES + h * B_HALF);
+          const uint32_t acc = tmem_base + ((x >> 1) & 1u) * BN + h * 128;
+          if (!early) ok = __all_sync(0xffffffffu, mbar_wait(&ready[slot], (x / (2 * STAGES)) & 1u, deadline, abort_flag));
+          if (!ok) break;
+          const uint32_t asked = x + 1 < total ? mbar_try_wait(&ready[next], ((x + 1) / (2 * STAGES)) & 1u) : 0u;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < BK / 32; ++k)
-                tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, BN), k != 0);
-              tc_commit(&done[stage]);
-            }
-            __syncwarp();
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1u;
-            }
+            for (int k = 0; k < BK / 32; ++k)
+              tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, 128), k != 0);
+            tc_commit(&done[slot]);
           }
+          early = __all_sync(0xffffffffu, asked);
         }
+        __syncwarp();
         if (elect_one()) tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
         __syncwarp();
         volatile int no_abort = 0;
@@ -284,14 +299,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
     const int half = (warp - EPI_BASE) >> 2;  // which half of the tile's columns
     const int row_in_tile = q * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(q * 32) << 16);
-    // this thread's two 64-column groups of the 256-column accumulator
-    const int col0 = SWIGLU ? 64 * half : 128 * half;
-    const int col1 = SWIGLU ? 128 + 64 * half : 128 * half + 64;
+    // this thread's two 64-column groups of the 256-column accumulator (SwiGLU: gate, then the up they meet)
+    const int col0 = 128 * half, col1 = 128 * half + 64;
     uint32_t it = 0, tcount = 0;
     bool ok = true;
     if (lane == 0) {  // both TMEM buffers start free
-      mbar_arrive(&ready[0]);
-      mbar_arrive(&ready[1]);
+      mbar_arrive(&ready[half]);
+      mbar_arrive(&ready[2 + half]);
     }
     for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x, ++tcount) {
       int m_t, n_t;
@@ -306,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
       for (int i = 0; i < 32; ++i) acc0[i] = acc1[i] = 0;
       // 64 columns are loaded while the 64 before them are folded, across K blocks as well
       uint32_t va[32], vb[32];
-      ok = warp_wait(&done[it % STAGES], (it / STAGES) & 1u, abort_flag);
+      ok = warp_wait(&done[2 * (it % STAGES) + half], (it / STAGES) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       tmem_ld_32x32b_x32(t_lane + (it & 1u) * BN + col0, va);
@@ -328,14 +342,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         fold32(acc0 + 16, vb, f0);
         tmem_ld_32x32b_x32(tb + col1 + 32, vb);
         // asked early: by the time the answer is used the next block is usually done
-        const bool early = more && mbar_try_wait(&done[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);
+        const bool early = more && mbar_try_wait(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u);
         tmem_wait_regs(va);
         tmem_wait_regs(vb);
         tc_fence_before();  // this warp's reads of the buffer are complete: K block it + 2 may have it
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ready[(it + 2) % STAGES]);
+        if (lane == 0) mbar_arrive(&ready[2 * ((it + 2) % STAGES) + half]);
         if (more && !__all_sync(0xffffffffu, early)) {
-          ok = warp_wait(&done[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u, abort_flag);
+          ok = warp_wait(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u, abort_flag);
           if (!ok) break;
         }
         tc_fence_after();

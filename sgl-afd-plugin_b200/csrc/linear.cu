@@ -230,6 +230,10 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
                             (uint64_t)L->KB * 128, BK, BM, "activation codes"))
     return rc;
   p.tmap_b = L->map;
+  if (swiglu && !L->d.atoms)  // boxes of 64 rows
+    if (int rc = make_tmap_2d(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (const void*)L->d.w, L->d.k, L->d.n, L->d.k, BK, 64,
+                              "gate and up weights"))
+      return rc;
   p.sa = (const float*)sa;
   p.sb = (const float*)L->d.scale;
   p.sfa = (const uint8_t*)sa;
