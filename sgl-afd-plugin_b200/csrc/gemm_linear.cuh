@@ -15,8 +15,8 @@
 //   is done the next one's scales have landed, and a folding warp reads them while its last fmas run;
 // - a K block is issued as two halves of 128 columns, each with its own barriers and its own four folding warps: one
 //   half's turn-around runs under the other's MMAs.  (Alone, MMAs of 128 columns take 710 cycles per K block, those of
-//   256 take 512; folded, 976 against 1009.)
-// 8192 x 8192 x 7168: 520 us = 1.85 PFLOP/s by itself.  In a row of launches the 1000 W cap sets the clock (1.65 GHz): 612
+//   256 take 512; folded, 950 against 1009.)
+// 8192 x 8192 x 7168: 505 us = 1.9 PFLOP/s by itself.  In a row of launches the 1000 W cap sets the clock (1.65 GHz): 600
 // us with the quantisation.
 #pragma once
 
@@ -88,6 +88,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     }
   }
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// A question to an mbarrier and its answer, apart: the answer stays in a predicate until it is asked for (in one statement
+// a selp behind the try_wait holds the warp up for the 200 cycles that the wait is to be hidden behind).  ASKED declares
+// the predicate, once in a kernel.
+#define ASKED() asm volatile(".reg .pred lin_asked;")
+__device__ __forceinline__ void ask(uint64_t* bar, uint32_t parity) {
+  asm volatile("mbarrier.try_wait.parity.shared::cta.b64 lin_asked, [%0], %1;" ::"r"(smem_u32(bar)), "r"(parity) : "memory");
+}
+__device__ __forceinline__ bool answer() {
+  uint32_t ok;
+  asm volatile("selp.u32 %0, 1, 0, lin_asked;" : "=r"(ok)::"memory");
+  return ok != 0;
 }
 
 // The same lane of a converged warp each time (the lane whose commits track its MMAs), as a predicate ptxas knows to be
@@ -170,6 +183,7 @@ __device__ __forceinline__ void store_rows(const uint32_t (&o)[16], uint8_t* wb,
 // h = silu(gate) * up, requantised per 1 x 128 (the tile's 128 h columns are one K block of the down product).
 template <int SWIGLU>
 __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_constant__ Params p) {
+  ASKED();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -275,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           const uint32_t acc = tmem_base + ((x >> 1) & 1u) * BN + h * 128;
           if (!early) ok = __all_sync(0xffffffffu, mbar_wait(&ready[slot], (x / (2 * STAGES)) & 1u, deadline, abort_flag));
           if (!ok) break;
-          const uint32_t asked = x + 1 < total ? mbar_try_wait(&ready[next], ((x + 1) / (2 * STAGES)) & 1u) : 0u;
+          ask(&ready[next], ((x + 1) / (2 * STAGES)) & 1u);
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -283,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
               tc_mma_f8f6f4(acc, adesc + 2ull * k, bdesc + 2ull * k, idesc_f8f6f4(BM, 128), k != 0);
             tc_commit(&done[slot]);
           }
-          early = __all_sync(0xffffffffu, asked);
+          early = __all_sync(0xffffffffu, answer());
         }
         __syncwarp();
         if (elect_one()) tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
@@ -342,13 +356,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         fold32(acc0 + 16, vb, f0);
         tmem_ld_32x32b_x32(tb + col1 + 32, vb);
         // asked early: by the time the answer is used the next block is usually done
-        const bool early = more && mbar_try_wait(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u);
+        ask(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u);
         tmem_wait_regs(va);
         tmem_wait_regs(vb);
         tc_fence_before();  // this warp's reads of the buffer are complete: K block it + 2 may have it
         __syncwarp();
         if (lane == 0) mbar_arrive(&ready[2 * ((it + 2) % STAGES) + half]);
-        if (more && !__all_sync(0xffffffffu, early)) {
+        if (!__all_sync(0xffffffffu, answer()) && more) {
           ok = warp_wait(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u, abort_flag);
           if (!ok) break;
         }
