@@ -43,8 +43,10 @@ def _check_logits(logits: torch.Tensor, scoring: str) -> None:
 def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """Logits whose rows are contiguous, and the row stride."""
     t, e = logits.shape
+    if logits.is_contiguous():
+        return logits, e
     if (e > 1 and logits.stride(1) != 1) or (t > 1 and logits.stride(0) < e):
-        logits = logits.contiguous()
+        return logits.contiguous(), e
     return logits, logits.stride(0) if t > 1 else e
 
 
@@ -65,8 +67,8 @@ def _route_forward(logits, opts):
     k, sigmoid, bias, groups, top_groups, renorm, scale, num_tokens = opts
     rows, ld = _rows(logits)
     t, e = rows.shape
-    ids = torch.empty((t, k), dtype=torch.int32, device=rows.device)
-    weights = torch.empty((t, k), dtype=torch.float32, device=rows.device)
+    ids = rows.new_empty((t, k), dtype=torch.int32)
+    weights = rows.new_empty((t, k), dtype=torch.float32)
     desc = N.Route_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, k, sigmoid, groups, top_groups, renorm, scale, 0,
                      0 if bias is None else bias.data_ptr(), 0 if num_tokens is None else num_tokens.data_ptr())
     if t:
@@ -122,9 +124,11 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: O
         if bias.dtype != torch.float32 or tuple(bias.shape) != (e,) or bias.device != logits.device:
             raise ValueError(f"bias must be float32 [{e}] on {logits.device}, got {bias.dtype} {tuple(bias.shape)} on "
                              f"{bias.device}")
-        bias = bias.detach().contiguous()
+        if not bias.is_contiguous():
+            bias = bias.detach().contiguous()
     if num_tokens is not None:
-        num_tokens = _device_int("num_tokens", num_tokens.reshape(-1), logits, (1,))
+        num_tokens = _device_int("num_tokens", num_tokens if num_tokens.dim() == 1 else num_tokens.reshape(-1), logits,
+                                 (1,))
     opts = (top_k, _SCORING[scoring], bias, num_groups, top_groups, int(renormalize), float(routed_scaling_factor),
             num_tokens)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -140,26 +144,29 @@ class _BalanceLoss(torch.autograd.Function):
         rows, ld = _rows(logits)
         t, e = rows.shape
         nbytes = N.lib().asap_balance_ws_bytes(t, seqs)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
-        counts = torch.empty((seqs, e), dtype=torch.int32, device=rows.device)
-        loss = torch.empty((), dtype=torch.float32, device=rows.device)
+        # the counts and, 8-byte aligned behind them, the workspace: one allocation, and one region to clear
+        pad = seqs * e & 1
+        buf = rows.new_empty(pad + seqs * e + (nbytes + 3) // 4, dtype=torch.int32)
+        counts = buf.as_strided((seqs, e), (e, 1), pad)
+        ws = buf.data_ptr() + 4 * (pad + seqs * e)
+        loss = rows.new_empty((), dtype=torch.float32)
         desc = N.Balance_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, ids.shape[1], sigmoid, seqs, coef, 0,
                            ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), counts.data_ptr())
         with _OnDevice(rows.get_device()) as stream:
-            N.run("asap_balance_loss", ctypes.byref(desc), ws.data_ptr(), nbytes, loss.data_ptr(), stream)
-        ctx.save_for_backward(rows, ids, ws, counts)
-        ctx.desc, ctx.nbytes = desc, nbytes
+            N.run("asap_balance_loss", ctypes.byref(desc), ws, nbytes, loss.data_ptr(), stream)
+        ctx.save_for_backward(rows, ids, buf, cu_seqlens)
+        ctx.desc, ctx.ws, ctx.nbytes = desc, ws, nbytes
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad_loss, _):
         _once(grad_loss)
-        rows, _, ws, _ = ctx.saved_tensors  # all of them: what changed since is refused
+        rows = ctx.saved_tensors[0]  # (unpacking refuses what has changed since, the counts among it)
         out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         grad = grad_loss.to(torch.float32).contiguous()
         with _OnDevice(rows.get_device()) as stream:
-            N.run("asap_balance_backward", ctypes.byref(ctx.desc), ws.data_ptr(), ctx.nbytes, grad.data_ptr(),
+            N.run("asap_balance_backward", ctypes.byref(ctx.desc), ctx.ws, ctx.nbytes, grad.data_ptr(),
                    out.data_ptr(), stream)
         return out, None, None, None, None, None
 

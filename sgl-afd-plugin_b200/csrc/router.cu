@@ -1122,8 +1122,13 @@ int asap_balance_loss(const asap_balance_t* b, uint64_t ws, uint64_t ws_bytes, u
     ASAP_CHECK_LAUNCH("balance_small_kernel");
     return ASAP_OK;
   }
-  ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, route::balance_ws(b->t, b->seqs).zeroed, st));
-  ASAP_CUDA(cudaMemsetAsync((void*)b->counts, 0, 4ull * b->seqs * b->e, st));
+  const uint64_t zeroed = route::balance_ws(b->t, b->seqs).zeroed, cells = 4ull * b->seqs * b->e;
+  if (b->counts + cells == ws) {
+    ASAP_CUDA(cudaMemsetAsync((void*)b->counts, 0, cells + zeroed, st));
+  } else {
+    ASAP_CUDA(cudaMemsetAsync((void*)ws, 0, zeroed, st));
+    ASAP_CUDA(cudaMemsetAsync((void*)b->counts, 0, cells, st));
+  }
   route::balance_count_kernel<<<(b->t + route::kCountRows - 1) / route::kCountRows, route::kCountThreads,
                                 4 * (b->e + 1), st>>>(a);
   ASAP_CHECK_LAUNCH("balance_count_kernel");
