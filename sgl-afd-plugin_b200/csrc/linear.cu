@@ -66,7 +66,7 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
     g = fminf(g, limit);
     u = fminf(fmaxf(u, -limit), limit);
   }
-  return g / (1.f + expf(-g)) * u;
+  return __fdividef(g, 1.f + expf(-g)) * u;  // within 2 ulp; a denominator above 2^126 gives 0, the value to 10^-36
 }
 
 }  // namespace lin
