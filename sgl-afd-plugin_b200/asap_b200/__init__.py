@@ -12,6 +12,10 @@ Reference API mirrored here:
   scheduler.py        FfnScheduler.run_job / rows_of, JobTimer       (srt/managers/scheduler.py)
   args.py             the --asap-* flags and transport_geometry()     (srt/arg_groups/fields/asap.py,
                                                                         srt/server_args.py)
+
+The attention rank's side of the layer beside it (SGLang's in the reference):
+  linear.py           Fp8Linear, Fp8SharedExpert: products by E4M3 weights with 128 x 128 block scales
+  router.py           route, balance_loss, expert_counts: the top-k choice, its balance and their gradients
 """
 
 __version__ = "0.1.0"

@@ -80,6 +80,8 @@ class _Weight:
             raise ValueError(f"{name}: the weight and its scales must be on one CUDA device")
         if w.data_ptr() % 16:
             raise ValueError(f"{name}: the weight must be 16-byte aligned")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{name}: a layer cannot be made while a CUDA graph is being captured")
         self.pow2 = scale.dtype == torch.float8_e8m0fnu
         self.w, self.scale = w, scale.float().contiguous()
         self.device = w.device
@@ -105,6 +107,11 @@ class _Weight:
             pass
 
 
+def _overlap(out: torch.Tensor, rows: torch.Tensor, ld: int, m: int, k: int) -> bool:
+    lo, hi = rows.data_ptr(), rows.data_ptr() + 2 * ((m - 1) * ld + k)
+    return m > 0 and out.data_ptr() < hi and lo < out.data_ptr() + out.numel() * out.element_size()
+
+
 def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int):
     """-> (x as rows the kernels can read, their stride, out of x's leading shape)."""
     if not weight.handle:
@@ -126,6 +133,8 @@ def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int)
         rows, ld = rows.clone(memory_format=torch.contiguous_format), weight.k
     if out is None:
         out = x.new_empty(shape)
+    elif _overlap(out, rows, ld, m, weight.k):
+        raise ValueError("out must not share memory with x")
     elif (out.dtype != x.dtype or tuple(out.shape) != shape or out.device != x.device or not out.is_contiguous()
           or out.data_ptr() % 16):
         raise ValueError(f"out must be a contiguous, 16-byte aligned {x.dtype} tensor of shape {shape} on {x.device}")

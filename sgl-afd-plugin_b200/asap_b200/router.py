@@ -57,10 +57,10 @@ def _device_int(name: str, x: torch.Tensor, like: torch.Tensor, shape) -> torch.
     return x.contiguous()
 
 
-def _once(grad: torch.Tensor) -> None:
+def _once() -> None:
     # backward runs with gradients enabled only under create_graph=True (torch's own guard costs 10 us a call)
-    if torch.is_grad_enabled() and grad.requires_grad:
-        raise RuntimeError("the router's gradients cannot be differentiated again")
+    if torch.is_grad_enabled():
+        raise RuntimeError("the router's gradients cannot be differentiated again (create_graph=True)")
 
 
 def _route_forward(logits, opts):
@@ -88,7 +88,7 @@ class _Route(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_weights, _):
-        _once(grad_weights)
+        _once()
         rows, ids = ctx.saved_tensors
         out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         if out.numel():
@@ -161,7 +161,7 @@ class _BalanceLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_loss, _):
-        _once(grad_loss)
+        _once()
         rows = ctx.saved_tensors[0]  # (unpacking refuses what has changed since, the counts among it)
         out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         grad = grad_loss.to(torch.float32).contiguous()

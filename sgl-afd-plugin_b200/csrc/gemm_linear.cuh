@@ -87,7 +87,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
       }
     }
   }
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  const bool all = __shfl_sync(0xffffffffu, ok, 0) != 0;
+  __syncwarp();  // what lane 0 acquired is every lane's
+  return all;
 }
 
 // A question to an mbarrier and its answer, apart: the answer stays in a predicate until it is asked for (in one statement

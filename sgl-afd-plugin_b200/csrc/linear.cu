@@ -445,6 +445,12 @@ int asap_fp8_linear_register(const asap_fp8_linear_t* d, uint64_t* handle) {
     set_error("asap_fp8_linear_register: out of host memory");
     return ASAP_EINVAL;
   }
+  // the kernels are loaded here, not by a first call that may be a captured one
+  if (int rc = lin::ensure_attrs()) {
+    delete L;
+    return rc;
+  }
+  for (int split = 1; split <= lin::SK_MAX_SPLIT; split *= 2) lin::clusters_at_once(split, false);
   L->d = *d;
   L->KB = (d->k + 127) / 128;
   L->NB = (d->n + 127) / 128;

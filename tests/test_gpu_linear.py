@@ -195,6 +195,52 @@ def test_linear_streams_and_graphs(cuda_ok, m):
     lin.check()
 
 
+FIRST_CALL_CAPTURED = """
+import torch
+from asap_b200.linear import Fp8Linear, Fp8SharedExpert
+from asap_b200.router import balance_loss, expert_counts, route
+gen = torch.Generator(device="cuda").manual_seed(0)
+w = 0.02 * torch.randn(256, 256, device="cuda", generator=gen)
+layer = Fp8Linear.from_float(w)
+shared = Fp8SharedExpert.from_float(w, 0.02 * torch.randn(256, 128, device="cuda", generator=gen))
+x = torch.randn({m}, 256, device="cuda", generator=gen).bfloat16()
+torch.cuda.synchronize()
+def run():
+    y = layer(x)
+    top = route(y, 8, scoring="sigmoid", bias=w[0])
+    loss, counts = balance_loss(y, top.topk_ids, scoring="sigmoid")
+    return y, shared(x), top.topk_weights, top.topk_ids, loss, counts, expert_counts(top.topk_ids, 256)
+g = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(g):
+    got = run()
+g.replay()
+torch.cuda.synchronize()
+with torch.no_grad():
+    want = run()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        Fp8Linear.from_float(w)
+except RuntimeError as e:
+    assert "being captured" in str(e), e
+else:
+    raise AssertionError("a layer was made in a capture")
+print("captured first")
+"""
+
+
+@pytest.mark.parametrize("m", [2, 600])
+def test_first_calls_of_a_process_may_be_captured(cuda_ok, m):
+    import os
+    import subprocess
+    import sys
+
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED.replace("{m}", str(m))], env=env, capture_output=True,
+                       text=True, timeout=120)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
 def test_linear_from_float_and_release(cuda_ok):
     gen = torch.Generator(device=DEV).manual_seed(0)
     layer = Fp8Linear.from_float(0.02 * torch.randn(256, 384, device=DEV, generator=gen))
@@ -226,6 +272,10 @@ def test_linear_refusals(cuda_ok):
                 torch.empty(128, 4, device=DEV, dtype=torch.bfloat16).t()):
         with pytest.raises(ValueError, match="out must be"):
             layer(x, out=out)
+    buf = torch.empty(4 * 256 + 4 * 128, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share memory"):
+        layer(buf[:1024].view(4, 256), out=buf[512:1024].view(4, 128))
+    layer(buf[:1024].view(4, 256).zero_(), out=buf[1024:].view(4, 128))
     with pytest.raises(ValueError, match="scales of shape"):
         Fp8Linear(w, s[:, :1])
     with pytest.raises(ValueError, match="scales of shape"):
