@@ -93,8 +93,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 // A question to an mbarrier and its answer, apart: the answer stays in a predicate until it is asked for (in one statement
-// a selp behind the try_wait holds the warp up for the 200 cycles that the wait is to be hidden behind).  ASKED declares
-// the predicate, once in a kernel.
+// a selp behind the try_wait holds the warp up for the 200 cycles that the wait is to be hidden behind).  Only of a phase
+// that will end: try_wait keeps the warp for some microseconds when it does not (test_wait would not, but loses 2 to 7% of
+// the product), so the last question is one whose answer is known.  ASKED declares the predicate, once in a kernel.
 #define ASKED() asm volatile(".reg .pred lin_asked;")
 __device__ __forceinline__ void ask(uint64_t* bar, uint32_t parity) {
   asm volatile("mbarrier.try_wait.parity.shared::cta.b64 lin_asked, [%0], %1;" ::"r"(smem_u32(bar)), "r"(parity) : "memory");
@@ -285,13 +286,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         const uint32_t total = (uint32_t)(num_tiles - (int)blockIdx.x + (int)gridDim.x - 1) / gridDim.x * (uint32_t)KB * 2u;
         bool ok = true, early = false;
         for (uint32_t x = 0; ok && x < total; ++x) {
-          const uint32_t slot = x % (2 * STAGES), stage = slot / 2, h = x & 1u, next = (x + 1) % (2 * STAGES);
+          const uint32_t slot = x % (2 * STAGES), stage = slot / 2, h = x & 1u, next = x + 1 < total ? x + 1 : x;
           const uint64_t adesc = sdesc_sw128(sA + stage * A_BYTES);
           const uint64_t bdesc = sdesc_sw128(sB + stage * B_BYTES + h * B_HALF);
           const uint32_t acc = tmem_base + ((x >> 1) & 1u) * BN + h * 128;
           if (!early) ok = __all_sync(0xffffffffu, mbar_wait(&ready[slot], (x / (2 * STAGES)) & 1u, deadline, abort_flag));
           if (!ok) break;
-          ask(&ready[next], ((x + 1) / (2 * STAGES)) & 1u);
+          ask(&ready[next % (2 * STAGES)], (next / (2 * STAGES)) & 1u);
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -358,7 +359,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
         fold32(acc0 + 16, vb, f0);
         tmem_ld_32x32b_x32(tb + col1 + 32, vb);
         // asked early: by the time the answer is used the next block is usually done
-        ask(&done[2 * ((it + 1) % STAGES) + half], ((it + 1) / STAGES) & 1u);
+        const uint32_t next = it + more;
+        ask(&done[2 * (next % STAGES) + half], (next / STAGES) & 1u);
         tmem_wait_regs(va);
         tmem_wait_regs(vb);
         tc_fence_before();  // this warp's reads of the buffer are complete: K block it + 2 may have it
