@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t atom_word(float pow2_scale) {
   return (__float_as_uint(pow2_scale) >> 23) * 0x01010101u;
 }
 
-template <int SWIGLU>
+template <int SWIGLU, bool SPLIT = false>
 __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -77,8 +77,11 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int KB = p.KB;
   const int num_tiles = p.m_tiles * p.n_tiles;
+  // with split > 1 a cluster has one tile, and this CTA the K blocks [kb0, kb0 + KB) of it
+  const int split = SPLIT ? p.split : 1, rank = SPLIT ? (int)cluster_rank() : 0;
+  const int kb0 = rank * p.KB / split, KB = (rank + 1) * p.KB / split - kb0;
+  const int tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
   const uint64_t deadline = globaltimer_ns() + p.timeout_ns;
 
   if (warp == 0) {
@@ -87,13 +90,13 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
         int m_t, n_t;
         decode_tile(p, tile, m_t, n_t);
         const int b0 = SWIGLU ? n_t * 128 : n_t * BN, b1 = SWIGLU ? p.N / 2 + n_t * 128 : n_t * BN + 128;
-        const uint8_t* sfa = p.sfa + (int64_t)m_t * KB * ATOM;
-        const uint8_t* sfb0 = p.sfb + (int64_t)(b0 / 128) * ATOM;
-        const uint8_t* sfb1 = p.sfb + (int64_t)(b1 / 128) * ATOM;
+        const uint8_t* sfa = p.sfa + ((int64_t)m_t * p.KB + kb0) * ATOM;
+        const uint8_t* sfb0 = p.sfb + ((int64_t)kb0 * p.nb_atoms + b0 / 128) * ATOM;
+        const uint8_t* sfb1 = p.sfb + ((int64_t)kb0 * p.nb_atoms + b1 / 128) * ATOM;
         for (int kb = 0; kb < KB; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, deadline, abort_flag)) {
             ok = false;
@@ -101,9 +104,9 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
           }
           uint8_t* sf = sSF + stage * 3 * ATOM;
           mbar_arrive_expect_tx(&full[stage], P2_STAGE_BYTES);
-          tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, kb * BK, m_t * BM, &full[stage]);
-          tma_load_2d(sB + stage * B_BYTES, &p.tmap_b, kb * BK, b0, &full[stage]);
-          tma_load_2d(sB + stage * B_BYTES + B_HALF, &p.tmap_b, kb * BK, b1, &full[stage]);
+          tma_load_2d(sA + stage * A_BYTES, &p.tmap_a, (kb0 + kb) * BK, m_t * BM, &full[stage]);
+          tma_load_2d(sB + stage * B_BYTES, &p.tmap_b, (kb0 + kb) * BK, b0, &full[stage]);
+          tma_load_2d(sB + stage * B_BYTES + B_HALF, &p.tmap_b, (kb0 + kb) * BK, b1, &full[stage]);
           bulk_load(sf, sfa + (int64_t)kb * ATOM, ATOM, &full[stage]);
           bulk_load(sf + ATOM, sfb0 + (int64_t)kb * p.nb_atoms * ATOM, ATOM, &full[stage]);
           bulk_load(sf + 2 * ATOM, sfb1 + (int64_t)kb * p.nb_atoms * ATOM, ATOM, &full[stage]);
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
     int stage = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+    for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
       ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, acc_phase ^ 1u, deadline, abort_flag));
       if (!ok) break;
       for (int kb = 0; kb < KB; ++kb) {
@@ -160,7 +163,8 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
     const int col0 = SWIGLU ? 64 * half : 128 * half;
     const int col1 = SWIGLU ? 128 + 64 * half : 128 * half + 64;
     uint32_t tcount = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++tcount) {
+    bool exchanged = false;
+    for (int tile = tile0; tile < num_tiles; tile += tile_step, ++tcount) {
       int m_t, n_t;
       decode_tile(p, tile, m_t, n_t);
       if (!warp_wait(acc_full, tcount & 1u, abort_flag)) break;
@@ -203,20 +207,43 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
                                          atom_off(row0 + lane, n_t, p.N / 256)) = atom_word(scale);
         }
       } else {
+        uint64_t a0[32], a1[32];  // pairs of columns
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          a0[i] = pair(__uint_as_float(v[i / 16][2 * (i % 16)]), __uint_as_float(v[i / 16][2 * (i % 16) + 1]));
+          a1[i] = pair(__uint_as_float(v[2 + i / 16][2 * (i % 16)]), __uint_as_float(v[2 + i / 16][2 * (i % 16) + 1]));
+        }
+        if constexpr (SPLIT) {  // the partials take the place of the operands, which every MMA is done with
+          exchange(a0, a1, reinterpret_cast<float*>(sA), split, rank, half, q * 32 + lane, true);
+          exchanged = true;
+        }
         uint8_t* wb = sOut + (warp - P2_EPI_BASE) * 2048;
         const int c0 = n_t * BN + half * 128;
         uint16_t* out0 = reinterpret_cast<uint16_t*>(p.out) + (int64_t)row0 * p.ldo + c0;
         const bool fp16 = p.out_fp16 != 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          if (SPLIT && !finishes(split, rank, half, c / 2)) continue;
+          const uint64_t* a = c < 2 ? a0 + 16 * c : a1 + 16 * (c - 2);
           uint32_t o[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            o[i] = pack16(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1]), fp16);
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = halves(a[i]);
+            o[i] = pack16(f.x, f.y, fp16);
+          }
           store_rows(o, wb, out0 + 32 * c, p.ldo, p.M - row0, p.N - c0 - 32 * c, lane);
         }
       }
     }
+    if (SPLIT && !exchanged) {  // this warp gave up: the cluster's barrier still counts it
+      __syncwarp();
+      cluster_sync();
+    }
+  }
+  if constexpr (SPLIT) {
+    __syncwarp();
+    if (warp < P2_EPI_BASE) cluster_sync();  // the exchange's barrier
+    cluster_leave();
   }
   tc_fence_before();
   __syncthreads();

@@ -45,22 +45,9 @@ struct SkinnyParams {
   uint64_t status, timeout_ns;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
 // Programmatic launch: wait until the kernels this one was launched beside have finished, and let the next one start.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ float4 peer_load4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -388,8 +375,7 @@ __global__ void __launch_bounds__(SK_THREADS, Skinny<TN, SWIGLU, XTMA>::C <= 32 
     }
   }
   tc_fence_before();
-  // no CTA leaves while another reads its shared memory; nothing is handed over, so the stores above need not be waited for
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+  cluster_leave();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, T::TMEM);

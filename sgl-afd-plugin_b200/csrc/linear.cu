@@ -152,8 +152,11 @@ static int ensure_attrs() {
   std::lock_guard<std::mutex> lk(mu);
   if (dev >= 0 && dev < 64 && done[dev]) return ASAP_OK;
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_gemm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
+  ASAP_CUDA(
+      cudaFuncSetAttribute(linear_pow2_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
   ASAP_CUDA(cudaFuncSetAttribute(linear_pow2_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, P2_SMEM_BYTES));
   for (const void* f : {(const void*)linear_skinny_kernel<16, 0, 0>, (const void*)linear_skinny_kernel<16, 0, 1>,
                         (const void*)linear_skinny_kernel<32, 0, 1>, (const void*)linear_skinny_kernel<64, 0, 1>,
@@ -220,6 +223,8 @@ static int quantise(uint64_t x, int64_t ldx, int32_t m, const Linear* L, int32_t
   return ASAP_OK;
 }
 
+static int tile_split(const Linear* L, bool swiglu, int32_t m);
+
 // One product over quantised activations.  swiglu: L holds gate rows then up rows, h goes to out_q / out_sa.
 static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32_t m, int64_t mp, uint64_t out,
                    int64_t ldo, int32_t fp16, float limit, uint64_t out_q, uint64_t out_sa, uint64_t status,
@@ -254,17 +259,23 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
   p.out_sa = (float*)out_sa;
   p.status = status;
   p.timeout_ns = timeout_ns;
+  p.split = tile_split(L, swiglu, m);
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
-  if (L->d.atoms) {
-    if (swiglu) linear_pow2_kernel<1><<<grid, P2_THREADS, P2_SMEM_BYTES, st>>>(p);
-    else linear_pow2_kernel<0><<<grid, P2_THREADS, P2_SMEM_BYTES, st>>>(p);
-    ASAP_CHECK_LAUNCH("linear_pow2_kernel");
-    return ASAP_OK;
-  }
-  if (swiglu) linear_gemm_kernel<1><<<grid, THREADS, SMEM_BYTES, st>>>(p);
-  else linear_gemm_kernel<0><<<grid, THREADS, SMEM_BYTES, st>>>(p);
-  ASAP_CHECK_LAUNCH("linear_gemm_kernel");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < sm_count() ? tiles : sm_count()));
+  cfg.blockDim = dim3(L->d.atoms ? P2_THREADS : THREADS);
+  cfg.dynamicSmemBytes = L->d.atoms ? P2_SMEM_BYTES : SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  void (*kernel)(Params) = L->d.atoms ? (swiglu ? linear_pow2_kernel<1> : linear_pow2_kernel<0>)
+                                      : (swiglu ? linear_gemm_kernel<1> : linear_gemm_kernel<0>);
+  if (p.split > 1) kernel = L->d.atoms ? linear_pow2_kernel<0, true> : linear_gemm_kernel<0, true>;
+  ASAP_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   return ASAP_OK;
 }
 
@@ -355,11 +366,28 @@ static SkinnyPlan skinny_plan(const Linear* L, int32_t m) {
   return SkinnyPlan{};
 }
 
-// The same measure of the product in 128 x 256 tiles.  A K block takes either kernel 0.6 to 0.7 us, so the one with fewer
-// rounds is taken: 7168 x 4096 with 256 rows 26.9 us against 39.4 (28 rounds, 56), with 384 rows 45.2 against 40.1 (56, 56).
-static int64_t tile_rounds(const Linear* L, bool swiglu, int32_t m) {
+// The product in 128 x 256 tiles: the CTAs of a cluster that share a tile's K blocks, where there are fewer tiles than SMs
+// and the K blocks saved are worth the exchange of the partials.  That takes 4 to 5 us, 10 K blocks' time: 7168 x 4096 with
+// 384 rows saves 28 blocks and 9.5 us; 2048 x 7168 with 160 rows (16 blocks) is the same shared or not, 17.5 us.  SwiGLU
+// needs a row's whole 128 h in one CTA and does not share.
+constexpr int kExchange = 10;
+static int64_t tile_rounds(const Linear* L, bool swiglu, int32_t m, int split) {
   const int64_t tiles = (int64_t)((m + BM - 1) / BM) * (swiglu ? L->d.n / 256 : (L->d.n + BN - 1) / BN);
+  if (split > 1 && (swiglu || split > L->KB || tiles > clusters_at_once(split, false))) return INT64_MAX;
+  if (split > 1) return (L->KB + split - 1) / split + kExchange;
   return (tiles + sm_count() - 1) / sm_count() * L->KB;
+}
+static int tile_split(const Linear* L, bool swiglu, int32_t m) {
+  int best = 1;
+  for (int s = 2; s <= 4; s *= 2)
+    if (tile_rounds(L, swiglu, m, s) < tile_rounds(L, swiglu, m, best)) best = s;
+  return best;
+}
+// The measure that chooses between tiles and few rows: a K block takes either kernel 0.4 to 0.7 us, so the one with fewer
+// rounds is taken.  7168 x 4096 with 256 rows: 24 rounds in shared tiles 25.4 us, 28 of the few-rows form 27.1, 56 in
+// tiles of one CTA 39.4.
+static int64_t tile_rounds(const Linear* L, bool swiglu, int32_t m) {
+  return tile_rounds(L, swiglu, m, tile_split(L, swiglu, m));
 }
 
 // What is the same for every launch of a call

@@ -113,6 +113,37 @@ def test_linear_against_the_definition(cuda_ok, m, k, n, scales, dtype):
     assert torch.equal(layer(x), y), "the same call gives the same bits"
 
 
+# Fewer 128 x 256 tiles than SMs and a long K: two or four CTAs share a tile's K blocks.  Whole and ragged tiles, K blocks
+# that do not divide (K = 5904: 47 of them), each on two streams at once and from a replayed graph.
+@pytest.mark.parametrize("scales,dtype", [("fp32", torch.bfloat16), ("fp32", torch.float16), ("e8m0", torch.bfloat16)])
+@pytest.mark.parametrize("m,k,n", [(384, 7168, 4096), (333, 5904, 4080), (640, 7168, 2048), (160, 7168, 4096),
+                                   (600, 7168, 1040), (601, 5904, 1040)])
+def test_linear_shares_a_tile_among_ctas(cuda_ok, m, k, n, scales, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(m + k + n)
+    w, s = weight(gen, n, k, scales)
+    layer = Fp8Linear(w, s)
+    x = hidden(gen, m, k, dtype)
+    y = layer(x)
+    lin.check()
+    check_linear(y, x, w, s)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    torch.cuda.synchronize()
+    for st in streams * 3:
+        with torch.cuda.stream(st):
+            outs.append(layer(x))
+    torch.cuda.synchronize()
+    wide = torch.full((m + 2, n), 7.0, dtype=dtype, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(x, out=wide[1:m + 1])
+    for _ in range(3):
+        graph.replay()
+    lin.check()
+    assert all(torch.equal(o, y) for o in outs) and torch.equal(wide[1:m + 1], y)
+    assert (wide[0] == 7).all() and (wide[m + 1] == 7).all()
+
+
 @pytest.mark.parametrize("m", [3, 40, 600])
 @pytest.mark.parametrize("scales", ["fp32", "e8m0"])
 def test_linear_takes_any_strides(cuda_ok, m, scales):
