@@ -153,12 +153,11 @@ def prepare(case, seed):
     gen = torch.Generator(device="cuda").manual_seed(1000003 * seed + 17)
     st = dict(case)
     dtype = _DTYPES[case.get("dtype", "bf16")]
-    if own:
-        _package()
     if case["op"] == "linear":
         st["x"] = _hidden(gen, case["m"], case["k"], dtype)
         st["w"], st["w_scale"] = _weight(gen, case["n"], case["k"], case["scales"])
         if own:
+            _package()
             from asap_b200.linear import Fp8Linear
             st["layer"] = Fp8Linear(st["w"], st["w_scale"])
     elif case["op"] == "shared":
@@ -166,6 +165,7 @@ def prepare(case, seed):
         st["w13"], st["w13_scale"] = _weight(gen, 2 * case["inter"], case["hidden"], case["scales"])
         st["w2"], st["w2_scale"] = _weight(gen, case["hidden"], case["inter"], case["scales"])
         if own:
+            _package()
             from asap_b200.linear import Fp8SharedExpert
             st["layer"] = Fp8SharedExpert(st["w13"], st["w13_scale"], st["w2"], st["w2_scale"],
                                           swiglu_limit=case["limit"])
