@@ -62,9 +62,9 @@ __device__ __forceinline__ void quant8(const uint4& u, bool fp16, bool pow2, uin
 }
 
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  if (limit > 0.f) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+  if (limit > 0.f) {  // by comparisons, which keep a NaN: fminf would give the limit
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
   }
   return __fdividef(g, 1.f + expf(-g)) * u;  // within 2 ulp; a denominator above 2^126 gives 0, the value to 10^-36
 }

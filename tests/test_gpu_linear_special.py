@@ -1,0 +1,29 @@
+"""What the FP8 linear and shared expert promise beside their values: special rows, streams, reloading, refusals."""
+
+import pytest
+import torch
+
+from asap_b200 import linear as lin
+from asap_b200.linear import Fp8Linear, Fp8SharedExpert
+from test_gpu_linear import hidden, weight
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("m", [6, 200, 9000])  # the few-rows kernels (16 and 64 columns wide), the 128 x 256 tiles
+@pytest.mark.parametrize("scales", ["fp32", "e8m0"])
+@pytest.mark.parametrize("limit", [0.0, 0.75])
+def test_shared_expert_special_rows_with_and_without_a_limit(cuda_ok, m, scales, limit):
+    gen = torch.Generator(device=DEV).manual_seed(m)
+    w13, s13 = weight(gen, 512, 384, scales)
+    w2, s2 = weight(gen, 384, 256, scales)
+    layer = Fp8SharedExpert(w13, s13, w2, s2, swiglu_limit=limit)
+    x = hidden(gen, m, 384, torch.bfloat16)
+    clean = layer(x)
+    assert clean.isfinite().all()
+    x[0, 1], x[1, 2], x[2, 380], x[3] = float("nan"), float("inf"), float("-inf"), 0.0
+    y = layer(x)
+    lin.check()
+    assert y[:3].isnan().all() and (y[3] == 0).all()
+    assert torch.equal(y[4:], clean[4:])
