@@ -63,6 +63,19 @@ def _once() -> None:
         raise RuntimeError("the router's gradients cannot be differentiated again (create_graph=True)")
 
 
+def _like(x: torch.Tensor) -> tuple:
+    return x.shape, x.dtype, x.device
+
+
+def _came_back(x: torch.Tensor, like: tuple) -> torch.Tensor:
+    """A saved tensor as backward may read it.  Its address is not the forward's: hooks unpack it elsewhere, and
+    checkpointing computes it again."""
+    if _like(x) != like:
+        raise RuntimeError(f"a tensor saved for the gradient came back as {x.dtype} {tuple(x.shape)} on {x.device}, was "
+                           f"{like[1]} {tuple(like[0])} on {like[2]}")
+    return x
+
+
 def _route_forward(logits, opts):
     k, sigmoid, bias, groups, top_groups, renorm, scale, num_tokens = opts
     rows, ld = _rows(logits)
@@ -82,16 +95,19 @@ class _Route(torch.autograd.Function):
     def forward(ctx, logits, opts):
         weights, ids, rows, desc = _route_forward(logits, opts)
         ctx.save_for_backward(rows, ids)
-        ctx.desc = desc
+        ctx.like = _like(rows), _like(ids)
+        ctx.desc = desc  # for its numbers: of its addresses, backward sets what it reads (the bias counts as given or not)
         ctx.mark_non_differentiable(ids)
         return weights, ids
 
     @staticmethod
     def backward(ctx, grad_weights, _):
         _once()
-        rows, ids = ctx.saved_tensors
+        rows, ids = map(_came_back, ctx.saved_tensors, ctx.like)
         out = torch.empty_like(rows, memory_format=torch.contiguous_format)
         if out.numel():
+            rows, ctx.desc.ld = _rows(rows)
+            ctx.desc.logits, ids = rows.data_ptr(), ids.contiguous()
             grad = grad_weights.to(torch.float32).contiguous()
             with _OnDevice(rows.get_device()) as stream:
                 N.run("asap_route_backward", ctypes.byref(ctx.desc), ids.data_ptr(), grad.data_ptr(), out.data_ptr(), stream)
@@ -148,26 +164,37 @@ class _BalanceLoss(torch.autograd.Function):
         pad = seqs * e & 1
         buf = rows.new_empty(pad + seqs * e + (nbytes + 3) // 4, dtype=torch.int32)
         counts = buf.as_strided((seqs, e), (e, 1), pad)
-        ws = buf.data_ptr() + 4 * (pad + seqs * e)
+        ctx.counts_at, ctx.ws_at = 4 * pad, 4 * (pad + seqs * e)  # bytes into buf
+        ws = buf.data_ptr() + ctx.ws_at
         loss = rows.new_empty((), dtype=torch.float32)
         desc = N.Balance_t(rows.data_ptr(), ld, _DTYPES[rows.dtype], t, e, ids.shape[1], sigmoid, seqs, coef, 0,
                            ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), counts.data_ptr())
         with _OnDevice(rows.get_device()) as stream:
             N.run("asap_balance_loss", ctypes.byref(desc), ws, nbytes, loss.data_ptr(), stream)
-        ctx.save_for_backward(rows, ids, buf, cu_seqlens)
-        ctx.desc, ctx.ws, ctx.nbytes = desc, ws, nbytes
+        saved = (rows, ids, buf) if cu_seqlens is None else (rows, ids, buf, cu_seqlens)
+        ctx.save_for_backward(*saved)
+        ctx.like = tuple(map(_like, saved))
+        ctx.desc, ctx.nbytes = desc, nbytes  # desc for its numbers: backward sets the addresses
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad_loss, _):
         _once()
-        rows = ctx.saved_tensors[0]  # (unpacking refuses what has changed since, the counts among it)
-        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
+        # (unpacking refuses what has changed since, the counts among it)
+        saved = tuple(map(_came_back, ctx.saved_tensors, ctx.like))
+        out = torch.empty_like(saved[0], memory_format=torch.contiguous_format)
+        rows, ctx.desc.ld = _rows(saved[0])
+        ids, buf, *cu = (x.contiguous() for x in saved[1:])
+        if buf.data_ptr() % 8:  # the workspace in it has 8-byte words
+            buf = buf.clone()
+        desc = ctx.desc
+        desc.logits, desc.ids, desc.counts = rows.data_ptr(), ids.data_ptr(), buf.data_ptr() + ctx.counts_at
+        desc.cu_seqlens = cu[0].data_ptr() if cu else 0
         grad = grad_loss.to(torch.float32).contiguous()
         with _OnDevice(rows.get_device()) as stream:
-            N.run("asap_balance_backward", ctypes.byref(ctx.desc), ctx.ws, ctx.nbytes, grad.data_ptr(),
-                   out.data_ptr(), stream)
+            N.run("asap_balance_backward", ctypes.byref(desc), buf.data_ptr() + ctx.ws_at, ctx.nbytes, grad.data_ptr(),
+                  out.data_ptr(), stream)
         return out, None, None, None, None, None
 
 
