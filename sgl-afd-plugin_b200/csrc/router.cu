@@ -553,6 +553,12 @@ __global__ void __launch_bounds__(32 * kWarps) route_back_kernel(const __grid_co
     }
   }
   float s, d[V];
+  if (!__any_sync(0xffffffffu, id >= 0)) {  // a padding row, or none left: nothing of its logits, which may be NaN, counts
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = 0.f;
+    store_row<V>(reinterpret_cast<uint8_t*>(p.out) + t * p.e * size, p.e, p.dtype, p.out_vec, lane, d);
+    return;
+  }
   if (p.sigmoid) {
     s = id >= 0 ? 1.f / (1.f + expf(-x)) : 0.f;
 #pragma unroll

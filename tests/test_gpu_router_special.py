@@ -54,3 +54,30 @@ def test_gradients_of_saved_tensors_that_come_back_elsewhere(cuda_ok, T, how, dt
     assert want.isfinite().all() and (want != 0).any()
     for _ in range(2):
         assert torch.equal(gradient(logits, how, cu, bias), want)
+
+
+# ---------------------------------------------------------------------------------------------------- special rows
+def weights_and_gradient(logits, scoring, renorm, biased, **kw):
+    T, E = logits.shape
+    x = logits.clone().requires_grad_(True)
+    bias = 0.01 * torch.arange(E, device=DEV, dtype=torch.float32) if biased else None
+    top = route(x, 6, scoring=scoring, renormalize=renorm, bias=bias, **kw)
+    grad = torch.randn(T, 6, device=DEV, generator=torch.Generator(device=DEV).manual_seed(T))
+    return top, torch.autograd.grad(top.topk_weights, x, grad)[0]
+
+
+@pytest.mark.parametrize("scoring,renorm,biased", FORMS)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf"), torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("E", [64, 72, 1000])
+def test_route_gradient_of_padding_rows(cuda_ok, E, value, scoring, renorm, biased):
+    """Rows behind the valid tokens have gradient 0 whatever they hold, and so has a row with no expert left."""
+    n = 30
+    clean = make_logits(40, E, torch.float32, E)
+    clean[4] = float("-inf")
+    logits = clean.clone()
+    logits[n:, 5], logits[33], logits[35, 40:] = value, value, value
+    top, dl = weights_and_gradient(logits, scoring, renorm, biased,
+                                   num_tokens=torch.tensor([n], dtype=torch.int32, device=DEV))
+    assert (top.topk_ids[n:] == -1).all() and (top.topk_weights[n:] == 0).all()
+    assert (dl[n:] == 0).all() and (dl[4] == 0).all()
+    assert dl[:n].isfinite().all() and (dl[:4] != 0).any(1).all()
