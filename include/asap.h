@@ -396,7 +396,8 @@ typedef struct {
 int asap_route(const asap_route_t* r, uint64_t ids, uint64_t weights, void* stream);
 
 /* d loss / d logits [t, e] of the logits' type, rows e apart, from grad_weights fp32 [t, k] and the ids asap_route
- * chose (the selection itself has no gradient; the bias gets none). */
+ * chose (the selection itself has no gradient; the bias gets none).  A row without an id gets 0, another row with a NaN
+ * logit NaN. */
 int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weights, uint64_t grad_logits,
                         void* stream);
 

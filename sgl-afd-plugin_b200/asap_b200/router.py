@@ -126,7 +126,8 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: O
 
     An expert whose logit is -inf is never chosen.  Places left over hold id -1 and weight 0, which the dispatch skips;
     so do all rows from ``num_tokens`` (int32 [1] on the device) on, the padding of a captured batch.  A row with a NaN
-    logit gets NaN weights.  The weights carry a gradient to the logits (not to the bias)."""
+    logit gets NaN weights.  The weights carry a gradient to the logits (not to the bias): 0 in rows that chose no
+    expert, NaN in other rows with a NaN logit."""
     _check_logits(logits, scoring)
     t, e = logits.shape
     if not 1 <= top_k <= min(e, MAX_TOPK):

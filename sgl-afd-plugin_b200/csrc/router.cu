@@ -523,7 +523,8 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? kRouteBlocks : 2) route_
 // w_j = c s_j / N with N = sum of the selected s + 1e-20 (1 without renormalisation).  ds_j = c / N (g_j - [renorm]
 // sum_i g_i s_i / N) on the selected experts; sigmoid: dl_j = s_j (1 - s_j) ds_j.  softmax: dl_e = s_e (ds_e - sum_i
 // ds_i s_i) for every e; after renormalisation that sum is c (sum g s) / N (1 - S / N), nothing unless S is of the size
-// of 1e-20, which only a bias can bring about: `dense` asks for the row.
+// of 1e-20, which only a bias can bring about: `dense` asks for the row's softmax.  Every form reads the row, for a NaN in
+// it: such a row's weights are NaN, so its gradient is NaN too, all of it.
 struct BackArgs {
   const void* logits;
   int64_t ld;
@@ -559,6 +560,11 @@ __global__ void __launch_bounds__(32 * kWarps) route_back_kernel(const __grid_co
     store_row<V>(reinterpret_cast<uint8_t*>(p.out) + t * p.e * size, p.e, p.dtype, p.out_vec, lane, d);
     return;
   }
+  load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, d);
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) nan |= d[i] != d[i];
+  nan = __any_sync(0xffffffffu, nan);
   if (p.sigmoid) {
     s = id >= 0 ? 1.f / (1.f + expf(-x)) : 0.f;
 #pragma unroll
@@ -566,7 +572,6 @@ __global__ void __launch_bounds__(32 * kWarps) route_back_kernel(const __grid_co
   } else {
     float z = 0.f, top;
     if (p.dense) {
-      load_row<V>(row, p.e, p.dtype, p.vec, lane, ninf, d);
       top = ninf;
 #pragma unroll
       for (int i = 0; i < V; ++i) top = fmaxf(top, d[i]);
@@ -608,6 +613,10 @@ __global__ void __launch_bounds__(32 * kWarps) route_back_kernel(const __grid_co
       for (int i = 0; i < V; ++i)
         if (e % V == i) d[i] += v;
     }
+  }
+  if (nan) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = __uint_as_float(0x7fc00000u);
   }
   store_row<V>(reinterpret_cast<uint8_t*>(p.out) + t * p.e * size, p.e, p.dtype, p.out_vec, lane, d);
 }

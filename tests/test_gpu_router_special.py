@@ -81,3 +81,20 @@ def test_route_gradient_of_padding_rows(cuda_ok, E, value, scoring, renorm, bias
     assert (top.topk_ids[n:] == -1).all() and (top.topk_weights[n:] == 0).all()
     assert (dl[n:] == 0).all() and (dl[4] == 0).all()
     assert dl[:n].isfinite().all() and (dl[:4] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("scoring,renorm,biased", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E", [16, 72, 1000])
+def test_route_gradient_of_a_nan_row_is_nan(cuda_ok, E, dtype, scoring, renorm, biased):
+    """As its weights are, in every form; a row of NaN alone chose nothing and has gradient 0."""
+    clean = make_logits(41, E, dtype, E)
+    want_top, want = weights_and_gradient(clean, scoring, renorm, biased)
+    logits = clean.clone()
+    logits[7, E - 1] = logits[20, 0] = float("nan")
+    logits[12] = float("nan")
+    top, dl = weights_and_gradient(logits, scoring, renorm, biased)
+    assert top.topk_weights[[7, 12, 20]].isnan().all() and (top.topk_ids[12] == -1).all()
+    assert dl[[7, 20]].isnan().all() and (dl[12] == 0).all()
+    rest = [r for r in range(41) if r not in (7, 12, 20)]
+    assert torch.equal(dl[rest], want[rest]) and torch.equal(top.topk_ids[rest], want_top.topk_ids[rest])
