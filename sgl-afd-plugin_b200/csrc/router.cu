@@ -221,10 +221,10 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
   const float ninf = __uint_as_float(0xff800000u);
   const float tol = !p.bias ? 0.f : p.sigmoid ? 8e-7f : 4e-6f;
   const bool refinable = p.sigmoid || !p.bias;  // a softmax takes its whole row
-  auto is_close = [&](uint32_t a, uint32_t b, float times) {  // keys a >= b, both open
+  auto is_close = [&](uint32_t a, uint32_t b) {  // keys a >= b, both open
     const float x = value_of(a & ~MASK);
     // (negated: two infinities are close)
-    return tol > 0.f ? !(x - value_of(b & ~MASK) >= times * (tol + fabsf(x) * kUlps)) : (a & ~MASK) == (b & ~MASK);
+    return tol > 0.f ? !(x - value_of(b & ~MASK) >= tol + fabsf(x) * kUlps) : (a & ~MASK) == (b & ~MASK);
   };
   my_id = -1;
   sort_descending<V>(key);
@@ -239,8 +239,12 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
     best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
     second = __shfl_sync(0xffffffffu, second, lane * lanes);
     const bool mine = lane < p.groups && best > kClosed;
-    float score = mine ? value_of(best & ~MASK) : ninf;
-    if (pairs && mine && second > kClosed) score += value_of(second & ~MASK);
+    float score = mine ? value_of(best & ~MASK) : ninf, size = fabsf(score);
+    if (pairs && mine && second > kClosed) {
+      const float other = value_of(second & ~MASK);
+      score += other;
+      size += fabsf(other);
+    }
     uint32_t k = mine ? key_of(score) : 0u, kept = 0, least = 0;
     for (int r = 0; r < p.top_groups; ++r) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, k);
@@ -252,9 +256,19 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
     }
     if (!TIES) {  // the least kept score against the best one dropped
       const uint32_t drop = __reduce_max_sync(0xffffffffu, k);
-      if (drop && is_close(least, drop, 2.f)) {
+      bool close = drop && !pairs && is_close(least, drop);
+      if (drop && pairs) {
+        // Each group's score is off by up to tol and the units of its two addends, which may be far larger than their sum:
+        // the least that a kept one can be against the most that a dropped one can.  (Negated: infinities are close.)
+        const float off = tol + size * kUlps;
+        const bool held = (kept >> lane) & 1u, sure = !mine || off < INFINITY;
+        const uint32_t low = __reduce_min_sync(0xffffffffu, mine && held ? key_of(score - off) : 0xffffffffu);
+        const uint32_t high = __reduce_max_sync(0xffffffffu, mine && !held ? key_of(score + off) : 0u);
+        close = low <= high || !__all_sync(0xffffffffu, sure);
+      }
+      if (close) {
         // a lane's two best, in 64 bits, unless the third may be one of them
-        const bool hard = V > 2 && key[V > 2 ? 2 : 0] > kClosed && is_close(key[V > 2 ? 1 : 0], key[V > 2 ? 2 : 0], 1.f);
+        const bool hard = V > 2 && key[V > 2 ? 2 : 0] > kClosed && is_close(key[V > 2 ? 1 : 0], key[V > 2 ? 2 : 0]);
         if (!refinable || __any_sync(0xffffffffu, hard)) return true;
         double a = -(double)INFINITY, b = a;
 #pragma unroll 1
@@ -301,7 +315,7 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
     } else {
       m = __reduce_max_sync(0xffffffffu, key[0]);
       if (j >= p.k) {
-        if (m <= kClosed || !is_close(prev, m, 1.f)) break;
+        if (m <= kClosed || !is_close(prev, m)) break;
         if (j == 32) return true;
       }
       src = __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1;
@@ -320,7 +334,7 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
   if (mine <= kClosed) my_id = -1;
   if (!TIES) {
     const uint32_t before = __shfl_up_sync(0xffffffffu, mine, 1);
-    if (__any_sync(0xffffffffu, lane > 0 && mine > kClosed && is_close(before, mine, 1.f))) {
+    if (__any_sync(0xffffffffu, lane > 0 && mine > kClosed && is_close(before, mine))) {
       if (!refinable) return true;
       const double d = my_id >= 0 ? exact_score(p, row, my_id) : -(double)INFINITY;
       int rank = 0, sorted = -1;

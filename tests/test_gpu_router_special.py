@@ -6,7 +6,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 from asap_b200.router import balance_loss, route
-from test_gpu_router import make_logits
+from test_gpu_router import check_route, make_logits
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -98,3 +98,31 @@ def test_route_gradient_of_a_nan_row_is_nan(cuda_ok, E, dtype, scoring, renorm, 
     assert dl[[7, 20]].isnan().all() and (dl[12] == 0).all()
     rest = [r for r in range(41) if r not in (7, 12, 20)]
     assert torch.equal(dl[rest], want[rest]) and torch.equal(top.topk_ids[rest], want_top.topk_ids[rest])
+
+
+# ------------------------------------------------------------------------------------------------------- the choice
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,E,big", [(200, 64, 16.0), (1000, 256, 16.0), (1000, 256, 1024.0), (300, 512, 1024.0),
+                                     (300, 256, 2.0 ** 20), (100, 256, 3.0e38)])
+def test_route_groups_whose_two_best_cancel(cuda_ok, T, E, big, scoring):
+    """One expert of a group far up and the rest far down: the group's sum is small, the rounding of its addends is not."""
+    logits = make_logits(T, E, torch.float32, E)
+    bias = torch.full((E,), -big, device=DEV)
+    bias[::E // 8] = big
+    for k in (4, 7):
+        check_route(logits, k, scoring=scoring, bias=bias, num_groups=8, top_groups=4)
+    bias[::E // 4] = 0.5  # every other group without such an expert: sums of two sizes
+    bias[1::E // 4] = 0.5
+    check_route(logits, 6, scoring=scoring, bias=bias, num_groups=8, top_groups=4)
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e9, torch.finfo(torch.float32).min, float("-inf")])
+def test_route_groups_of_experts_biased_away(cuda_ok, low):
+    """A rank's experts switched off by a very negative bias: whole groups, and all but one of a group."""
+    E = 256
+    logits = make_logits(200, E, torch.float32, 9)
+    bias = 0.1 * torch.randn(E, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    bias[32:96] = low
+    bias[129:160] = low
+    for scoring in ("sigmoid", "softmax"):
+        check_route(logits, 8, scoring=scoring, bias=bias, num_groups=8, top_groups=4)
