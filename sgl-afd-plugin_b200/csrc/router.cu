@@ -206,6 +206,7 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[V]) {
 // two scores within tol + |score| (V + 2) 2^-23 of each other: tol for how the scores were computed (0: they are exact), V
 // units in the last place for the place bits, two for the sum with the bias.
 constexpr uint32_t kClosed = 0x007fffffu;  // the key of -inf
+constexpr uint32_t kTwo = 0xc0000000u;     // the key of 2
 
 // score + bias of one expert (a sigmoid), or its logit, in 64 bits
 __device__ __noinline__ double exact_score(const Args& p, const void* row, int e) {
@@ -214,7 +215,7 @@ __device__ __noinline__ double exact_score(const Args& p, const void* row, int e
 }
 
 template <int V, bool TIES>
-__device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const void* row, int lane, int& my_id) {
+__device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const void* row, int lane, bool& nan, int& my_id) {
   constexpr uint32_t MASK = Place<V>::MASK;
   constexpr float kUlps = (V + 2) * 1.1920929e-7f;
   const bool pairs = !TIES && p.bias;
@@ -228,6 +229,9 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
   };
   my_id = -1;
   sort_descending<V>(key);
+  // two questions to the warp in one: a NaN in the row, a score above 2
+  const uint32_t any = __reduce_or_sync(0xffffffffu, (nan ? 1u : 0u) | (key[0] > kTwo ? 2u : 0u));
+  nan = any & 1u;
   if (p.groups > 1) {  // a group is an aligned run of lanes
     const int lanes = 1 << p.group_log_lanes;
     uint32_t best = key[0], second = V > 1 ? key[V > 1 ? 1 : 0] : 0u;
@@ -239,12 +243,8 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
     best = __shfl_sync(0xffffffffu, best, lane * lanes);  // lane g: group g (lanes >= groups: unused)
     second = __shfl_sync(0xffffffffu, second, lane * lanes);
     const bool mine = lane < p.groups && best > kClosed;
-    float score = mine ? value_of(best & ~MASK) : ninf, size = fabsf(score);
-    if (pairs && mine && second > kClosed) {
-      const float other = value_of(second & ~MASK);
-      score += other;
-      size += fabsf(other);
-    }
+    float score = mine ? value_of(best & ~MASK) : ninf;
+    if (pairs && mine && second > kClosed) score += value_of(second & ~MASK);
     uint32_t k = mine ? key_of(score) : 0u, kept = 0, least = 0;
     for (int r = 0; r < p.top_groups; ++r) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, k);
@@ -258,13 +258,18 @@ __device__ __forceinline__ bool choose(const Args& p, uint32_t (&key)[V], const 
       const uint32_t drop = __reduce_max_sync(0xffffffffu, k);
       bool close = drop && !pairs && is_close(least, drop);
       if (drop && pairs) {
-        // Each group's score is off by up to tol and the units of its two addends, which may be far larger than their sum:
-        // the least that a kept one can be against the most that a dropped one can.  (Negated: infinities are close.)
-        const float off = tol + size * kUlps;
-        const bool held = (kept >> lane) & 1u, sure = !mine || off < INFINITY;
-        const uint32_t low = __reduce_min_sync(0xffffffffu, mine && held ? key_of(score - off) : 0xffffffffu);
-        const uint32_t high = __reduce_max_sync(0xffffffffu, mine && !held ? key_of(score + off) : 0u);
-        close = low <= high || !__all_sync(0xffffffffu, sure);
+        // A group's score is off by tol and the units of its two addends.  Unless one is above 2, they cannot cancel, and
+        // are at most |score| + 4; then the order of the scores is in doubt only next to the border.
+        const float x = value_of(least);
+        close = (any & 2u) || !(x - value_of(drop) >= 2.f * (tol + (fabsf(x) + 4.f) * kUlps));
+        if (close) {  // the least that a kept one can be against the most that a dropped one can
+          const float size = fabsf(value_of(best & ~MASK)) + (second > kClosed ? fabsf(value_of(second & ~MASK)) : 0.f);
+          const float off = tol + size * kUlps;
+          const bool held = (kept >> lane) & 1u, sure = off < INFINITY;  // else it may be anything
+          const uint32_t low = __reduce_min_sync(0xffffffffu, mine && held ? sure ? key_of(score - off) : 0u : 0xffffffffu);
+          const uint32_t high = __reduce_max_sync(0xffffffffu, mine && !held ? sure ? key_of(score + off) : 0xffffffffu : 0u);
+          close = low <= high;
+        }
       }
       if (close) {
         // a lane's two best, in 64 bits, unless the third may be one of them
@@ -491,7 +496,6 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? kRouteBlocks : 2) route_
     float top = ninf, z = 1.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) nan |= l[i] != l[i];
-    nan = __any_sync(0xffffffffu, nan);
     if (!p.sigmoid) {
 #pragma unroll
       for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
@@ -505,7 +509,9 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? kRouteBlocks : 2) route_
     int id;
     uint32_t key[V];
     bool unsure = !p.aligned_groups;
-    if (!unsure) {
+    if (unsure) {
+      nan = __any_sync(0xffffffffu, nan);
+    } else {
       float b[V];
       const float rz = 1.f / z;
       if (!TIES && p.bias)
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? kRouteBlocks : 2) route_
         x = fmaxf(l[i] > ninf ? x : ninf, ninf);  // NaN is closed
         key[i] = (key_of(x) & ~MASK) | (MASK - i);
       }
-      unsure = choose<V, TIES>(p, key, row, lane, id);
+      unsure = choose<V, TIES>(p, key, row, lane, nan, id);
     }
     if (unsure) id = choose_exactly<V>(p, row, lane);
     float s = 0.f;
