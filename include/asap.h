@@ -405,7 +405,7 @@ int asap_route_backward(const asap_route_t* r, uint64_t ids, uint64_t grad_weigh
  * f_e P_e, f_e = e / (k n) * count_e, P_e = mean of p_te over the sequence's n live tokens (those with an id), p the
  * row's softmax or its sigmoids normalised to sum 1.  ids int32 [t, k], -1: none.  cu_seqlens int32 [seqs + 1] on the
  * device, from 0, not decreasing (0: one sequence); tokens behind the last sequence do not take part.  counts int32
- * [seqs, e] is written; the gradient reads it and the workspace again.  The loss is the same bits every time. */
+ * [seqs, e] is written; the gradient reads it and the workspace again, ids and cu_seqlens not.  The loss is the same bits every time. */
 typedef struct {
   uint64_t logits;
   int64_t ld;

@@ -63,16 +63,12 @@ def _once() -> None:
         raise RuntimeError("the router's gradients cannot be differentiated again (create_graph=True)")
 
 
-def _like(x: torch.Tensor) -> tuple:
-    return x.shape, x.dtype, x.device
-
-
-def _came_back(x: torch.Tensor, like: tuple) -> torch.Tensor:
+def _came_back(x: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """A saved tensor as backward may read it.  Its address is not the forward's: hooks unpack it elsewhere, and
     checkpointing computes it again."""
-    if _like(x) != like:
+    if x.shape != shape or x.dtype is not dtype or x.device != device:
         raise RuntimeError(f"a tensor saved for the gradient came back as {x.dtype} {tuple(x.shape)} on {x.device}, was "
-                           f"{like[1]} {tuple(like[0])} on {like[2]}")
+                           f"{dtype} {shape} on {device}")
     return x
 
 
@@ -95,22 +91,25 @@ class _Route(torch.autograd.Function):
     def forward(ctx, logits, opts):
         weights, ids, rows, desc = _route_forward(logits, opts)
         ctx.save_for_backward(rows, ids)
-        ctx.like = _like(rows), _like(ids)
-        ctx.desc = desc  # for its numbers: of its addresses, backward sets what it reads (the bias counts as given or not)
+        # for its numbers: of its addresses, backward sets those that it reads (the bias only counts as given or not)
+        ctx.desc, ctx.kind = desc, (rows.dtype, rows.device)
         ctx.mark_non_differentiable(ids)
         return weights, ids
 
     @staticmethod
     def backward(ctx, grad_weights, _):
         _once()
-        rows, ids = map(_came_back, ctx.saved_tensors, ctx.like)
+        rows, ids = ctx.saved_tensors
+        desc, (dtype, device) = ctx.desc, ctx.kind
+        t, e = desc.t, desc.e
+        ids = _came_back(ids, (t, desc.k), torch.int32, device).contiguous()
+        rows, desc.ld = _rows(_came_back(rows, (t, e), dtype, device))
         out = torch.empty_like(rows, memory_format=torch.contiguous_format)
-        if out.numel():
-            rows, ctx.desc.ld = _rows(rows)
-            ctx.desc.logits, ids = rows.data_ptr(), ids.contiguous()
+        if t:
+            desc.logits = rows.data_ptr()
             grad = grad_weights.to(torch.float32).contiguous()
-            with _OnDevice(rows.get_device()) as stream:
-                N.run("asap_route_backward", ctypes.byref(ctx.desc), ids.data_ptr(), grad.data_ptr(), out.data_ptr(), stream)
+            with _OnDevice(device.index) as stream:
+                N.run("asap_route_backward", ctypes.byref(desc), ids.data_ptr(), grad.data_ptr(), out.data_ptr(), stream)
         return out, None
 
 
@@ -172,28 +171,25 @@ class _BalanceLoss(torch.autograd.Function):
                            ids.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), counts.data_ptr())
         with _OnDevice(rows.get_device()) as stream:
             N.run("asap_balance_loss", ctypes.byref(desc), ws, nbytes, loss.data_ptr(), stream)
-        saved = (rows, ids, buf) if cu_seqlens is None else (rows, ids, buf, cu_seqlens)
-        ctx.save_for_backward(*saved)
-        ctx.like = tuple(map(_like, saved))
-        ctx.desc, ctx.nbytes = desc, nbytes  # desc for its numbers: backward sets the addresses
+        ctx.save_for_backward(rows, buf)  # the workspace says which tokens count, and where: ids and offsets are not needed
+        # for its numbers: of its addresses, backward sets those that it reads
+        ctx.desc, ctx.nbytes, ctx.kind = desc, nbytes, (buf.numel(), rows.dtype, rows.device)
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad_loss, _):
         _once()
-        # (unpacking refuses what has changed since, the counts among it)
-        saved = tuple(map(_came_back, ctx.saved_tensors, ctx.like))
-        out = torch.empty_like(saved[0], memory_format=torch.contiguous_format)
-        rows, ctx.desc.ld = _rows(saved[0])
-        ids, buf, *cu = (x.contiguous() for x in saved[1:])
-        if buf.data_ptr() % 8:  # the workspace in it has 8-byte words
+        rows, buf = ctx.saved_tensors  # (refuses what has changed since, the counts among it)
+        desc, (words, dtype, device) = ctx.desc, ctx.kind
+        rows, desc.ld = _rows(_came_back(rows, (desc.t, desc.e), dtype, device))
+        buf = _came_back(buf, (words,), torch.int32, device).contiguous()
+        if buf.data_ptr() & 7:  # the workspace in it has 8-byte words
             buf = buf.clone()
-        desc = ctx.desc
-        desc.logits, desc.ids, desc.counts = rows.data_ptr(), ids.data_ptr(), buf.data_ptr() + ctx.counts_at
-        desc.cu_seqlens = cu[0].data_ptr() if cu else 0
+        out = torch.empty_like(rows, memory_format=torch.contiguous_format)
+        desc.logits, desc.counts = rows.data_ptr(), buf.data_ptr() + ctx.counts_at
         grad = grad_loss.to(torch.float32).contiguous()
-        with _OnDevice(rows.get_device()) as stream:
+        with _OnDevice(device.index) as stream:
             N.run("asap_balance_backward", ctypes.byref(desc), buf.data_ptr() + ctx.ws_at, ctx.nbytes, grad.data_ptr(),
                   out.data_ptr(), stream)
         return out, None, None, None, None, None
