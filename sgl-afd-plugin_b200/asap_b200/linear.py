@@ -29,7 +29,7 @@ import torch
 from . import _native as N
 
 MAX_ROWS = 1 << 20
-TIMEOUT_NS = 5_000_000_000  # bound of every wait inside the kernels
+TIMEOUT_NS = 5_000_000_000  # what the waits inside the kernels have, counted from their start
 _status: dict = {}          # device index -> int64 status word
 
 

@@ -71,28 +71,6 @@ __device__ __forceinline__ uint64_t sdesc_sw128(const void* p) {
   return ((a >> 4) & 0x3FFFull) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// A bounded wait of a whole warp: one lane polls, every lane gets its answer and the warp is converged after it.  (With
-// 32 lanes polling, the folding and scale warps filled the shared-memory pipe: a wait on a barrier that had long
-// completed then took the MMA issuer 210 cycles, three of them per K block.)  It ends when another warp's wait has run
-// out (the producer and the MMA issuer watch the clock) or after kSpins tries, some seconds: a count is an immediate, a
-// deadline would hold two registers that the folding warps do not have.
-constexpr uint32_t kSpins = 1u << 27;
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) {
-    for (uint32_t it = 0; ok && !mbar_try_wait(bar, parity);) {
-      ++it;
-      if ((it & 255u) == 0 && (*abort || it > kSpins)) {
-        *abort = 1;
-        ok = 0;
-      }
-    }
-  }
-  const bool all = __shfl_sync(0xffffffffu, ok, 0) != 0;
-  __syncwarp();  // what lane 0 acquired is every lane's
-  return all;
-}
-
 // A question to an mbarrier and its answer, apart: the answer stays in a predicate until it is asked for (in one statement
 // a selp behind the try_wait holds the warp up for the 200 cycles that the wait is to be hidden behind).  Only of a phase
 // that will end: try_wait keeps the warp for some microseconds when it does not (test_wait would not, but loses 2 to 7% of
@@ -384,10 +362,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_gemm_kernel(const __grid_co
           early = __all_sync(0xffffffffu, answer());
         }
         __syncwarp();
-        if (elect_one()) tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
+        if (elect_one()) tc_commit(mma_done);
         __syncwarp();
-        volatile int no_abort = 0;
-        mbar_wait(mma_done, 0, globaltimer_ns() + 200000000ull, &no_abort);
+        drain_mmas(mma_done, deadline, abort_flag);
       }
     }
   } else {

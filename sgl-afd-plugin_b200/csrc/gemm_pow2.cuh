@@ -151,10 +151,9 @@ __global__ void __launch_bounds__(P2_THREADS, 1) linear_pow2_kernel(const __grid
       }
       acc_phase ^= 1u;
     }
-    if (elect_one()) tc_commit(mma_done);  // every MMA issued has completed before TMEM is released
+    if (elect_one()) tc_commit(mma_done);
     __syncwarp();
-    volatile int no_abort = 0;
-    mbar_wait(mma_done, 0, globaltimer_ns() + 200000000ull, &no_abort);
+    drain_mmas(mma_done, deadline, abort_flag);
   } else {
     // ---------------- epilogue
     const int q = warp & 3;                      // TMEM lane quarter this warp may access

@@ -235,8 +235,7 @@ __global__ void __launch_bounds__(SK_THREADS, Skinny<TN, SWIGLU, XTMA>::C <= 32 
     }
     if (elect_one()) tc_commit(mma_done);
     __syncwarp();
-    volatile int no_abort = 0;
-    mbar_wait(mma_done, 0, globaltimer_ns() + 200000000ull, &no_abort);
+    drain_mmas(mma_done, deadline, abort_flag);
   } else {
     const int fw = warp - 2, ft = threadIdx.x - 64;
     for (int i = ft; i < kbs; i += 32 * SK_FOLD_WARPS) {

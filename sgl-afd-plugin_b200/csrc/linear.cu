@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "tmap.cuh"
+#include "waits.cuh"
 
 namespace asap {
 
