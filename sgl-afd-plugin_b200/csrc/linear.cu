@@ -62,10 +62,23 @@ __device__ __forceinline__ void quant8(const uint4& u, bool fp16, bool pow2, uin
   codes = make_uint2(codes4(v, inv), codes4(v + 4, inv));
 }
 
+// fminf and fmaxf would give the limit for a NaN; these give the NaN.  (So do two comparisons, but they spill in the fold
+// kernel: 2% of a shared expert of 16384 tokens.)
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  if (limit > 0.f) {  // by comparisons, which keep a NaN: fminf would give the limit
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : u < -limit ? -limit : u;
+  if (limit > 0.f) {
+    g = min_nan(g, limit);
+    u = min_nan(max_nan(u, -limit), limit);
   }
   return __fdividef(g, 1.f + expf(-g)) * u;  // within 2 ulp; a denominator above 2^126 gives 0, the value to 10^-36
 }
