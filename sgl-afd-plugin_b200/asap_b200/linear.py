@@ -30,25 +30,50 @@ from . import _native as N
 
 MAX_ROWS = 1 << 20
 TIMEOUT_NS = 5_000_000_000  # what the waits inside the kernels have, counted from their start
-_status: dict = {}          # device index -> int64 status word
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
-    word = _status.get(device.index)
-    if word is None:
-        word = _status[device.index] = torch.zeros(1, dtype=torch.int64, device=device)
-    return word
+class _Status:
+    """A word of pinned host memory in which a kernel reports that it gave up a wait: the host reads it with a plain
+    load."""
 
+    def __init__(self):
+        self.tensor = torch.zeros(1, dtype=torch.int64, pin_memory=True)
+        self.word = ctypes.c_uint64.from_address(self.tensor.data_ptr())
+        self.ptr = self.tensor.data_ptr()
 
-def check(device: int = 0) -> None:
-    """Raise if a kernel of this module gave up a wait on ``device`` (synchronises it)."""
-    word = _status.get(device)
-    if word is not None:
-        torch.cuda.synchronize(device)
-        value = int(word.item())
+    def check(self) -> None:
+        value = self.word.value
         if value:
-            word.zero_()
-            raise N.AsapError("asap_fp8_linear", N.ASAP_ETIMEOUT, f"device status {N.decode_status(value)}")
+            self.word.value = 0
+            raise N.AsapError("asap_fp8_linear", N.ASAP_ETIMEOUT, f"a kernel gave up a wait and its call's result is "
+                              f"garbage; device status {N.decode_status(value)}")
+
+
+_status: dict = {}  # device index -> _Status
+
+
+def _status_of(device: torch.device) -> _Status:
+    status = _status.get(device.index)
+    if status is None:
+        status = _status[device.index] = _Status()
+    return status
+
+
+def poll(device: Optional[int] = None) -> None:
+    """Raise if a kernel of this module has reported by now that it gave up a wait on ``device`` (None: on any).  Does
+    not wait for kernels under way.  Every later call of a layer on that device does the same, and so does
+    ``AttnChannel.check``, which the round trip calls for every message."""
+    for index, status in list(_status.items()):
+        if device is None or index == device:
+            status.check()
+
+
+def check(device: Optional[int] = None) -> None:
+    """``poll`` after everything enqueued on ``device`` (None: on every device that has a layer) has run."""
+    for index in list(_status):
+        if device is None or index == device:
+            torch.cuda.synchronize(index)
+    poll(device)
 
 
 def _scale_atoms(scale: torch.Tensor) -> torch.Tensor:
@@ -86,6 +111,8 @@ class _Weight:
         self.w, self.scale = w, scale.float().contiguous()
         self.device = w.device
         self.atoms = _scale_atoms(scale) if self.pow2 else None
+        self.reports = _status_of(self.device)
+        self.status = self.reports.ptr
         self.handle = 0
         desc = N.Fp8Linear_t(self.n, self.k, self.w.data_ptr(), self.scale.data_ptr(),
                              self.atoms.data_ptr() if self.pow2 else 0)
@@ -93,7 +120,6 @@ class _Weight:
         with torch.cuda.device(self.device):
             N.call("asap_fp8_linear_register", ctypes.byref(desc), ctypes.byref(h))
         self.handle = h.value
-        self.status = _status_word(self.device).data_ptr()
 
     def release(self) -> None:
         if self.handle:
@@ -116,6 +142,8 @@ def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int)
     """-> (x as rows the kernels can read, their stride, out of x's leading shape)."""
     if not weight.handle:
         raise RuntimeError("the layer was released")
+    if weight.reports.word.value:
+        weight.reports.check()
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] != weight.k or x.get_device() != weight.device.index:

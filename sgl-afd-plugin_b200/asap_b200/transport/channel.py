@@ -29,6 +29,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import _native as N
+from .. import linear
 from .layout import PROTO_VERSION, SEQ_MASK, ChannelPoisoned, Geometry, HandshakeError
 from .memory import Shared
 from .memory import select as select_memory
@@ -206,7 +207,8 @@ class AttnChannel:
 
     # ---------------------------------------------------------------- failure state
     def check(self) -> None:
-        """Raise ChannelPoisoned if a device wait ran out (the reference's watchdog semantics)."""
+        """Raise ChannelPoisoned if a device wait ran out (the reference's watchdog semantics); AsapError if a wait of an
+        FP8 linear or shared expert on this device did (the channel itself is sound then)."""
         if self._poison is None and self.status is not None:
             word = self.status.read()
             if word:
@@ -217,6 +219,7 @@ class AttnChannel:
                     "are garbage until reconnect()")
         if self._poison is not None:
             raise self._poison
+        linear.poll(self.device)
 
     @property
     def result_base(self) -> int:

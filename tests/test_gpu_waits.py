@@ -7,6 +7,7 @@ import shutil
 import subprocess
 
 import pytest
+import torch
 
 pytestmark = pytest.mark.gpu
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sgl-afd-plugin_b200", "csrc")
@@ -45,6 +46,16 @@ __global__ void waits(int arrive, uint64_t timeout_ns, uint64_t* out) {
   }
 }
 
+__global__ void tell(uint64_t status, uint64_t word) {
+  report(status, word);
+  report(status, word + 1);  // the first report stays
+}
+
+extern "C" int run_tell(uint64_t status, uint64_t word) {
+  tell<<<1, 1>>>(status, word);
+  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
+}
+
 extern "C" int run(int arrive, uint64_t timeout_ns, uint64_t* host) {
   uint64_t* dev = nullptr;
   if (cudaMalloc(&dev, 24) != cudaSuccess) return 1;
@@ -73,7 +84,28 @@ def run(cuda_ok, tmp_path_factory):
         assert lib.run(ctypes.c_int(arrive), ctypes.c_uint64(timeout_ns), out) == 0
         return bool(out[0]), bool(out[1]), out[2] / 1e9
 
+    call.lib = lib
     return call
+
+
+def test_a_report_reaches_the_next_call(run):
+    """A kernel's report in the word that the layers give theirs: the next call raises it, once."""
+    from asap_b200 import _native as N
+    from asap_b200 import linear
+
+    x = torch.randn(4, 256, device="cuda").bfloat16()
+    layer = linear.Fp8Linear.from_float(torch.randn(128, 256, device="cuda"))
+    want = layer(x)
+    linear.check()
+    word = 5 | (18 << 32)  # pipeline timeout
+    assert run.lib.run_tell(ctypes.c_uint64(layer._w.status), ctypes.c_uint64(word)) == 0
+    with pytest.raises(N.AsapError, match="gave up a wait"):
+        layer(x)
+    assert torch.equal(layer(x), want)
+    assert run.lib.run_tell(ctypes.c_uint64(layer._w.status), ctypes.c_uint64(word)) == 0
+    with pytest.raises(N.AsapError, match="'seq': 18"):
+        linear.check()
+    linear.check()
 
 
 def test_waits_that_are_over(run):
