@@ -58,6 +58,15 @@ class AsapDispatcher(BaseDispatcher):
             return out if shared is None else out + shared
         return AsapBuffer.get().recv(combine_input.ticket, shared=shared)
 
+    def abandon(self, combine_input: AsapDispatchOutput) -> None:
+        """Take the replies of a message whose combine will not come (what was to be added to it raised) and drop them:
+        the message's tensors are let go of only behind the work that reads them, and its slot is as after a combine."""
+        if combine_input.ticket is not None:
+            try:
+                AsapBuffer.get().recv(combine_input.ticket)
+            except Exception as e:  # noqa: BLE001  (the caller has an exception to raise already)
+                logger.warning(f"[ASAP] the replies to {combine_input.ticket} could not be taken: {e}")
+
 
 class AsapBuffer:
     """The attention rank's channel to the FFN ranks (asap.py:81-206)."""

@@ -56,4 +56,9 @@ class AsapMoE(torch.nn.Module):
         dispatch_output = self.dispatcher.dispatch(hidden_states, topk_output)
         if self.shared_expert is None:
             return self.dispatcher.combine(dispatch_output)
-        return self.dispatcher.combine(dispatch_output, shared=self.shared_expert(hidden_states))
+        try:
+            shared = self.shared_expert(hidden_states)
+            return self.dispatcher.combine(dispatch_output, shared=shared)
+        except BaseException:
+            self.dispatcher.abandon(dispatch_output)
+            raise

@@ -5,7 +5,9 @@ import torch
 
 from asap_b200 import linear as lin
 from asap_b200.linear import Fp8Linear, Fp8SharedExpert
+from asap_b200.router import route
 from test_gpu_linear import hidden, weight
+from test_gpu_moe_layer import layer  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -27,3 +29,20 @@ def test_shared_expert_special_rows_with_and_without_a_limit(cuda_ok, m, scales,
     lin.check()
     assert y[:3].isnan().all() and (y[3] == 0).all()
     assert torch.equal(y[4:], clean[4:])
+
+
+def test_layer_after_its_shared_expert_refused(layer):
+    """The message that was out is taken back: the layer's next calls, on every slot, are as before."""
+    lb, moe_layer, gate, _ = layer
+    x = torch.randn(40, moe_layer.hidden_size, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4)).bfloat16()
+    with torch.no_grad():
+        topk = route(gate(x)[:, :16], 4)
+        want = moe_layer(x, topk)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            moe_layer(x.clone().requires_grad_(True), topk)
+    with torch.no_grad():
+        for _ in range(3):
+            assert torch.equal(moe_layer(x, topk), want)
+    torch.cuda.synchronize()
+    lb.check()
