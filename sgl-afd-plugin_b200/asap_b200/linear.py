@@ -25,6 +25,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -133,6 +134,11 @@ class _Weight:
             pass
 
 
+def _has_tangent(x: torch.Tensor) -> bool:
+    """Forward-mode differentiation: the kernels would drop the tangent without a word."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 def _overlap(out: torch.Tensor, rows: torch.Tensor, ld: int, m: int, k: int) -> bool:
     lo, hi = rows.data_ptr(), rows.data_ptr() + 2 * ((m - 1) * ld + k)
     return m > 0 and out.data_ptr() < hi and lo < out.data_ptr() + out.numel() * out.element_size()
@@ -150,6 +156,8 @@ def _rows(x: torch.Tensor, weight: _Weight, out: Optional[torch.Tensor], n: int)
         raise ValueError(f"x must be [..., {weight.k}] on {weight.device}, got {tuple(x.shape)} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the FP8 products have no gradient: call them under torch.no_grad() or detach x")
+    if _has_tangent(x):
+        raise RuntimeError("the FP8 products have no forward-mode gradient: detach x")
     shape = (*x.shape[:-1], n)
     rows = x if x.dim() == 2 else x.reshape(-1, weight.k)
     m, ld = rows.shape[0], weight.k

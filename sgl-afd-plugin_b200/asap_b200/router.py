@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as N
-from .linear import _OnDevice
+from .linear import _has_tangent, _OnDevice
 from .sglang_shim import StandardTopKOutput
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -38,6 +38,8 @@ def _check_logits(logits: torch.Tensor, scoring: str) -> None:
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
     if not 1 <= logits.shape[1] <= MAX_EXPERTS:
         raise ValueError(f"need 1 to {MAX_EXPERTS} experts, got {logits.shape[1]}")
+    if _has_tangent(logits):
+        raise RuntimeError("the router and the balance loss have no forward-mode gradient: detach the logits")
 
 
 def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int]:

@@ -2,10 +2,11 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from asap_b200 import linear as lin
 from asap_b200.linear import Fp8Linear, Fp8SharedExpert
-from asap_b200.router import route
+from asap_b200.router import balance_loss, route
 from test_gpu_linear import hidden, weight
 from test_gpu_moe_layer import layer  # noqa: F401  (a fixture)
 
@@ -46,3 +47,21 @@ def test_layer_after_its_shared_expert_refused(layer):
             assert torch.equal(moe_layer(x, topk), want)
     torch.cuda.synchronize()
     lb.check()
+
+
+def test_forward_mode_tangents_are_refused(cuda_ok):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    linear = Fp8Linear(*weight(gen, 128, 256, "fp32"))
+    shared = Fp8SharedExpert(*weight(gen, 256, 256, "fp32"), *weight(gen, 256, 128, "fp32"))
+    x, t = hidden(gen, 4, 256, torch.bfloat16), hidden(gen, 4, 256, torch.bfloat16)
+    l, ids = torch.randn(4, 8, device=DEV, generator=gen), torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    with fwAD.dual_level():
+        dual, dual_l = fwAD.make_dual(x, t), fwAD.make_dual(l, torch.ones_like(l))
+        for call in (lambda: linear(dual), lambda: shared(dual), lambda: route(dual_l, 2), lambda: balance_loss(dual_l, ids),
+                     lambda: linear(dual[1:]), lambda: route(dual_l.clone().requires_grad_(True), 2)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(linear(dual.detach()), linear(x)) and torch.equal(linear(x), linear(x))
+        assert torch.equal(route(dual_l.detach(), 2).topk_ids, route(l, 2).topk_ids)
