@@ -112,6 +112,8 @@ class _Weight:
         self.w, self.scale = w, scale.float().contiguous()
         self.device = w.device
         self.atoms = _scale_atoms(scale) if self.pow2 else None
+        # what was laid out here, or by from_float, may be read on any stream from now on
+        torch.cuda.current_stream(self.device).synchronize()
         self.reports = _status_of(self.device)
         self.status = self.reports.ptr
         self.handle = 0

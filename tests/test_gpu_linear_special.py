@@ -65,3 +65,32 @@ def test_forward_mode_tangents_are_refused(cuda_ok):
                 call()
         assert torch.equal(linear(dual.detach()), linear(x)) and torch.equal(linear(x), linear(x))
         assert torch.equal(route(dual_l.detach(), 2).topk_ids, route(l, 2).topk_ids)
+
+
+@pytest.mark.parametrize("m", [3, 2000])
+@pytest.mark.parametrize("made", ["e8m0", "strided", "from_float"])
+def test_layer_made_on_a_busy_stream_serves_another(cuda_ok, made, m):
+    """What a layer lays out of its scales is there when it has been made, whatever stream calls it first."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    dense = 0.02 * torch.randn(512, 1024, device=DEV, generator=gen)
+    w, s = weight(gen, 512, 1024, "fp32" if made == "strided" else "e8m0")
+    wide = s.float().repeat_interleave(2, 1)  # the scales as every other column
+
+    def make():
+        if made == "from_float":
+            return Fp8Linear.from_float(dense)
+        return Fp8Linear(w, wide[:, ::2] if made == "strided" else s)
+
+    x = hidden(gen, m, 1024, torch.bfloat16)
+    want = make()(x)
+    torch.cuda.synchronize()
+    for n in (8 * 4 * 512, 4 * 8 * 4, 512 * 1024):  # what the layer's own tensors will be made of
+        torch.full((n,), 90, dtype=torch.uint8, device=DEV)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)  # some 60 ms of the current stream
+    layer = make()
+    with torch.cuda.stream(other):
+        y = layer(x)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
