@@ -15,8 +15,11 @@ Activations are quantised inside the call, per row and block b of 128 values alo
 * E8M0 weight scales (``torch.float8_e8m0fnu``): sa = amax / 448 rounded up to a power of two, xq = e4m3(x / sa).
 
 amax counts as at least 1e-10.  A NaN or infinity in a row makes that row of the result NaN and no other.  Sums are
-held in fp32 and rounded once to x's type.  Both are for serving: they have no gradient.  A call allocates its scratch
-from torch's caching allocator on the current stream, so calls on different streams and captured graphs share nothing.
+held in fp32 and rounded once to x's type.  Both are for serving: they have no gradient.
+
+A layer reads the weight tensor it was made of where it is and may hold its scales as a copy: after writing new values
+into them call ``reload``.  A call allocates its scratch from torch's caching allocator on the current stream, so calls on
+different streams and captured graphs share nothing.
 """
 
 from __future__ import annotations
@@ -109,7 +112,7 @@ class _Weight:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{name}: a layer cannot be made while a CUDA graph is being captured")
         self.pow2 = scale.dtype == torch.float8_e8m0fnu
-        self.w, self.scale = w, scale.float().contiguous()
+        self.w, self.given, self.scale = w, scale, scale.float().contiguous()  # scale: given's memory, or a copy
         self.device = w.device
         self.atoms = _scale_atoms(scale) if self.pow2 else None
         # what was laid out here, or by from_float, may be read on any stream from now on
@@ -123,6 +126,12 @@ class _Weight:
         with torch.cuda.device(self.device):
             N.call("asap_fp8_linear_register", ctypes.byref(desc), ctypes.byref(h))
         self.handle = h.value
+
+    def reload(self) -> None:
+        if self.scale.data_ptr() != self.given.data_ptr():
+            self.scale.copy_(self.given)
+        if self.pow2:
+            self.atoms.copy_(_scale_atoms(self.given))
 
     def release(self) -> None:
         if self.handle:
@@ -236,6 +245,12 @@ class Fp8Linear:
                       ws.data_ptr() if nbytes else 0, nbytes, w.status, TIMEOUT_NS, stream)
         return out
 
+    def reload(self) -> None:
+        """To be called after new values were written into the weight and scale tensors this layer was made of: the weight
+        is read where it is, and so are contiguous fp32 scales, but of others the layer holds copies.  Renewed in place on
+        the current stream, so that captured graphs see them too."""
+        self._w.reload()
+
     def release(self) -> None:
         self._w.release()
 
@@ -273,6 +288,11 @@ class Fp8SharedExpert:
                 N.run("asap_fp8_shared", a.handle, b.handle, rows.data_ptr(), ld, m, x.dtype == torch.float16,
                       self.swiglu_limit, out.data_ptr(), ws.data_ptr(), nbytes, a.status, TIMEOUT_NS, stream)
         return out
+
+    def reload(self) -> None:
+        """As ``Fp8Linear.reload``, for both weights."""
+        self._w13.reload()
+        self._w2.reload()
 
     def release(self) -> None:
         self._w13.release()

@@ -94,3 +94,30 @@ def test_layer_made_on_a_busy_stream_serves_another(cuda_ok, made, m):
         y = layer(x)
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("m", [3, 40, 2500])
+@pytest.mark.parametrize("scales", ["fp32", "strided", "e8m0"])
+def test_reload_after_new_values_in_place(cuda_ok, scales, m):
+    gen = torch.Generator(device=DEV).manual_seed(m)
+    kind = "e8m0" if scales == "e8m0" else "fp32"
+    old, new = [[weight(gen, 512, 256, kind), weight(gen, 256, 256, kind)] for _ in range(2)]
+    if scales == "strided":
+        old = [(w, s.t().contiguous().t()) for w, s in old]
+    (w13, s13), (w2, s2) = old
+    layer, shared = Fp8Linear(w13, s13), Fp8SharedExpert(w13, s13, w2, s2)
+    x = hidden(gen, m, 256, torch.bfloat16)
+    first = layer(x), shared(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = layer(x), shared(x)
+    for (w, s), (v, t) in zip(old, new):
+        w.view(torch.uint8).copy_(v.view(torch.uint8))
+        s.copy_(t)
+    layer.reload()
+    shared.reload()
+    want = Fp8Linear(*new[0])(x), Fp8SharedExpert(*new[0], *new[1])(x)
+    graph.replay()
+    for a, b, c, d in zip((layer(x), shared(x)), want, captured, first):
+        assert torch.equal(a, b) and torch.equal(c, b) and not torch.equal(a, d)
+    lin.check()
