@@ -161,7 +161,10 @@ struct Args {
   const void* logits;
   int64_t ld;
   int32_t dtype, t, e, k, sigmoid, groups, top_groups, renorm, vec;
-  int32_t aligned_groups;  // a group is a whole number of lanes, a power of two of them (or there is one group)
+  // A group is a whole number of lanes, a power of two of them (or there is one group): the fast choice, whose shuffles
+  // reduce a group.  Other groupings rank every row from the start in 64 bits, right and slow: 16384 x 160 in 8 groups
+  // (V = 8, 20 experts a group) with a bias 101 us, in one group 16; 16384 x 256 in 8 groups 18.
+  int32_t aligned_groups;
   int32_t group_log_lanes;
   float scale;
   const float* bias;         // NULL: none
@@ -744,7 +747,8 @@ __global__ void __launch_bounds__(kCountThreads) balance_count_kernel(const __gr
   }
 }
 
-// p_e of a row, and q_e = 1 - sigmoid(l_e) with sigmoids.  A row of sigmoids whose largest logit is negative is scaled by
+// p_e of a row, and q_e = 1 - sigmoid(l_e) with sigmoids, whose quotients are approximate (2 units in the last place, as the
+// exponential before them).  A row of sigmoids whose largest logit is negative is scaled by
 // e^-top, so that its values do not underflow before they are normalised.
 template <int V>
 __device__ __forceinline__ void row_probabilities(bool sigmoid, float (&l)[V], float (&p)[V], float (&q)[V]) {
@@ -863,8 +867,15 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 4 : 2) balance_kernel(co
 }
 
 // A few tokens in one block and one launch: the counts, sequences and factors as balance_count_kernel leaves them, and the
-// loss.  8 tokens x 256 experts: 5.0 us against 11 for a memset, the counts and the loss; 512 x 16: 14.9 against 11.0, but
-// 24 us of the caller's time against 30, which is what such a call waits for; 1024 x 16: 26.6 against 13.8.
+// loss.  Against a memset, the counts and the loss the caller saves two launches, 21 us of its time for 25; on the GPU (us,
+// here / there) it wins while one block keeps up:
+//   16 experts:  16 tokens  3.8 /  9.7, 192  7.8 / 11.1, 320 10.7 / 12.1, 384 12.1 / 11.9, 512 15.0 / 11.5, 768 20.9 / 11.8
+//   64:          16 tokens  4.2 / 11.2, 128  6.7 / 11.6, 256  9.9 / 12.4, 384 13.2 / 12.4, 512 16.5 / 12.4
+//   256:         16 tokens  5.1 / 11.9,  64  8.2 / 13.1, 128 12.9 / 13.0, 192 17.6 / 14.0
+//   1000:        16 tokens 17.3 / 19.3,  32 29.2 / 20.3
+// Taken where what the GPU loses is no more than the 4 us that the caller saves, for every number of experts: tokens x V up
+// to 512 (the widest margin is left with 64 to 512 experts, the least with 16 and 512 tokens, where a captured graph loses
+// 3.5 us and an eager call gains 4).
 constexpr int kSmallWarps = 32, kSmallTokens = 512, kSmallCounts = 4096;  // tokens x V; sequences x experts
 template <int V>
 __global__ void __launch_bounds__(32 * kSmallWarps) balance_small_kernel(const __grid_constant__ BalanceArgs p) {

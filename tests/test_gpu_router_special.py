@@ -6,7 +6,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 from asap_b200.router import balance_loss, route
-from test_gpu_router import check_route, make_logits
+from test_gpu_router import check_balance, check_route, make_logits
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -126,3 +126,15 @@ def test_route_groups_of_experts_biased_away(cuda_ok, low):
     bias[129:160] = low
     for scoring in ("sigmoid", "softmax"):
         check_route(logits, 8, scoring=scoring, bias=bias, num_groups=8, top_groups=4)
+
+
+# ----------------------------------------------------------------------------------------------------- balance loss
+@pytest.mark.parametrize("T,E,k", [(511, 16, 2), (512, 16, 2), (256, 64, 6), (257, 64, 6), (128, 128, 6), (129, 128, 6),
+                                   (64, 256, 8), (32, 512, 8), (33, 512, 8), (16, 1000, 8), (17, 1000, 8)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_balance_around_the_single_launch(cuda_ok, T, E, k, scoring):
+    """The last sizes of the single launch and the first of the three."""
+    logits = make_logits(T, E, torch.float32, T + E)
+    ids = route(logits, k, scoring=scoring).topk_ids
+    check_balance(logits, ids, scoring)
+    check_balance(logits, ids, scoring, cu=torch.tensor([0, 5, 5, T - 3], dtype=torch.int32, device=DEV))
