@@ -295,7 +295,8 @@ static int product(const Linear* L, bool swiglu, uint64_t xq, uint64_t sa, int32
 
 // ------------------------------------------------------------------ few rows
 // Up to here the few-rows linear quantises its rows itself.  7168 x 4096: 1 row 10.8 us against 11.0 with a kernel before
-// it (2064 x 1040: 5.3 against 5.8), and one launch less for the caller; 8 rows 13.1 against 11.7.
+// it (2064 x 1040: 5.3 against 5.8), and one launch less for the caller; 8 rows 13.1 against 11.7.  Only the linear: the
+// shared expert's rows come quantised from the first one on, as its second product's do.
 constexpr int kInKernelRows = 4;
 constexpr int kInKernelDim = SK_MAX_KB * SK_MAX_SPLIT * BK;  // and this many values of K, whose codes fit the clusters
 
