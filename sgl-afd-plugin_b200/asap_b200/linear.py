@@ -112,6 +112,7 @@ class _Weight:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{name}: a layer cannot be made while a CUDA graph is being captured")
         self.pow2 = scale.dtype == torch.float8_e8m0fnu
+        w, scale = w.detach(), scale.detach()  # parameters may require a gradient; the layer has none
         self.w, self.given, self.scale = w, scale, scale.float().contiguous()  # scale: given's memory, or a copy
         self.device = w.device
         self.atoms = _scale_atoms(scale) if self.pow2 else None

@@ -103,7 +103,7 @@ def test_reload_after_new_values_in_place(cuda_ok, scales, m):
     kind = "e8m0" if scales == "e8m0" else "fp32"
     old, new = [[weight(gen, 512, 256, kind), weight(gen, 256, 256, kind)] for _ in range(2)]
     if scales == "strided":
-        old = [(w, s.t().contiguous().t()) for w, s in old]
+        old = [(w, s.t().contiguous().t().requires_grad_(True)) for w, s in old]  # as a parameter may
     (w13, s13), (w2, s2) = old
     layer, shared = Fp8Linear(w13, s13), Fp8SharedExpert(w13, s13, w2, s2)
     x = hidden(gen, m, 256, torch.bfloat16)
@@ -111,13 +111,15 @@ def test_reload_after_new_values_in_place(cuda_ok, scales, m):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         captured = layer(x), shared(x)
-    for (w, s), (v, t) in zip(old, new):
-        w.view(torch.uint8).copy_(v.view(torch.uint8))
-        s.copy_(t)
+    with torch.no_grad():
+        for (w, s), (v, t) in zip(old, new):
+            w.view(torch.uint8).copy_(v.view(torch.uint8))
+            s.copy_(t)
     layer.reload()
     shared.reload()
     want = Fp8Linear(*new[0])(x), Fp8SharedExpert(*new[0], *new[1])(x)
     graph.replay()
     for a, b, c, d in zip((layer(x), shared(x)), want, captured, first):
         assert torch.equal(a, b) and torch.equal(c, b) and not torch.equal(a, d)
+    assert not layer._w.scale.requires_grad and layer._w.scale.grad_fn is None  # no history grows with every reload
     lin.check()
